@@ -474,6 +474,80 @@ int uocr_kv_state(uocr_ctx *ctx, const uocr_kv *kv, size_t seq, size_t *tokens, 
 int uocr_kv_export(uocr_ctx *ctx, const uocr_kv *kv, size_t seq, float *keys_out,
                    float *values_out, size_t *tokens);
 
+/* ---- KV cache held in 4 or 8 bits --------------------------------------------
+ * No counterpart in the reference, whose caches hold floats.  uocr_kvq is
+ * uocr_kv (the same prefix and ring, slots, counters and order of calls) with
+ * every 32 consecutive dims of one head of one token's key or value (a group;
+ * the last of a head may be short) held as codes of `bits` bits (4 or 8), a
+ * step s and a least value m (bf16 each): bits + 1 bits a dim at whole groups,
+ * against 32.  With L = 2^bits - 1:
+ *   m = the largest bf16 <= min x, s = the smallest bf16 >= (max x - m) / L,
+ *   code = clamp(rint((x - m) / s), 0, L), 0 where s is 0
+ * (differences and quotients in double, rint half to even); it stands for
+ * m + s * code, which is within s / 2 of x.  A value that is not finite, or of
+ * magnitude 2^100 and above, is Numerical at the next synchronising call and
+ * its group reads as NaN.  head_dim <= 256, any; device rows of heads * head_dim
+ * floats, ld_* floats apart (0: next to each other), of any alignment.  A cache
+ * belongs to the device of the context that created it (Invalid with a context
+ * of another device) and is used by one stream at a time; all calls but create,
+ * free and state are asynchronous on the context's stream, allocate nothing and
+ * can be captured in CUDA graphs.
+ *   uocr_kvq_prefill:  the rows of a prompt into the empty sequence seq;
+ *   uocr_kvq_push:     row b of k/v into every sequence b;
+ *   uocr_kvq_rope, uocr_kvq_rope_push_qkv: as uocr_kv_rope and
+ *                      uocr_kv_rope_push_qkv;
+ *   uocr_kvq_attention: softmax(q . K / sqrt(head_dim)) V of q row b over the
+ *                      tokens of sequence b and what the cache stands for, FP32
+ *                      accumulation (FP32 tolerance); a row of q that is not
+ *                      finite, or scores that are not, give NaN outputs for that
+ *                      head and Numerical at the next synchronising call;
+ *   uocr_kvq_read:     what slots [first, first + count) of sequence seq stand
+ *                      for, as token-major rows of floats (a head's slots lie in
+ *                      the physical order of uocr_kv); slots past its tokens are
+ *                      Shape at the next synchronising call at the latest, their
+ *                      rows left as they were;
+ *   uocr_kvq_state, uocr_kvq_reset: as for uocr_kv;
+ *   uocr_kvq_storage_bytes: device bytes of the codes and parameters.
+ * push / rope / attention before every sequence is prefilled: Shape. */
+typedef struct uocr_kvq uocr_kvq;
+int uocr_kvq_create(uocr_ctx *ctx, size_t batch, size_t heads, size_t head_dim, size_t window,
+                    size_t max_prefix, int bits, uocr_kvq **out);
+int uocr_kvq_free(uocr_kvq *kv);
+size_t uocr_kvq_storage_bytes(const uocr_kvq *kv);
+int uocr_kvq_reset(uocr_ctx *ctx, uocr_kvq *kv, size_t seq);
+int uocr_kvq_prefill(uocr_ctx *ctx, uocr_kvq *kv, size_t seq, const float *keys_dev, size_t ld_keys,
+                     const float *values_dev, size_t ld_values, size_t tokens);
+int uocr_kvq_push(uocr_ctx *ctx, uocr_kvq *kv, const float *k_dev, size_t ld_k, const float *v_dev,
+                  size_t ld_v);
+int uocr_kvq_rope(uocr_ctx *ctx, const uocr_kvq *kv, const uocr_rope *rope, float *q_dev,
+                  float *k_dev);
+int uocr_kvq_rope_push_qkv(uocr_ctx *ctx, uocr_kvq *kv, const uocr_rope *rope, const float *qkv_dev,
+                           float *q_out_dev);
+int uocr_kvq_attention(uocr_ctx *ctx, const uocr_kvq *kv, const float *q_dev, float *out_dev);
+int uocr_kvq_state(uocr_ctx *ctx, const uocr_kvq *kv, size_t seq, size_t *tokens, size_t *position);
+int uocr_kvq_read(uocr_ctx *ctx, const uocr_kvq *kv, size_t seq, size_t first, size_t count,
+                  float *keys_out_dev, float *values_out_dev);
+
+/* ---- log probabilities of tokens ------------------------------------------------
+ * What rows of logits say of given tokens (no counterpart in the reference,
+ * which takes the largest): rows of vocab floats, ld floats apart (0: next to
+ * each other).  With p = softmax of the row, in natural logarithms:
+ *   logprob[r]  = log p(tokens[r]); 0 where tokens[r] is negative (a row without
+ *                 a token); tokens and logprob may be NULL together;
+ *   entropy[r]  = -sum p log p (may be NULL);
+ *   top_ids / top_logprobs [rows x top_k]: the top_k largest logits, larger
+ *                 first, equal ones by the lower id, and their log p
+ *                 (top_k <= 32 and <= vocab; 0: none).
+ * -inf is a logit of probability 0 (a banned token).  A row that holds NaN or
+ * +inf, or nothing but -inf, gives NaN (ids -1) and Numerical at the next
+ * synchronising call; a token id of vocab or above NaN and Shape.  Sums in FP32,
+ * the maximum's own term kept apart, so that a nearly certain token's log
+ * probability and a nearly zero entropy keep an FP32 relative precision.
+ * Asynchronous on the context's stream; allocates nothing. */
+int uocr_token_logprobs(uocr_ctx *ctx, const float *logits_dev, size_t rows, size_t vocab, size_t ld,
+                        const int64_t *tokens_dev, size_t top_k, float *logprob_dev,
+                        float *entropy_dev, int64_t *top_ids_dev, float *top_logprobs_dev);
+
 /* ---- INT8 overlay (QuantizedWeights) --------------------------------------
  * The "uocr-q8-block32-v1" overlay: a safetensors file holding, for every
  * projection matrix of the source checkpoint, "<name>" (I8 [rows, cols]) and

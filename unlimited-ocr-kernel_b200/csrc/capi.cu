@@ -13,6 +13,7 @@
 #include <cstdio>
 #include <cstring>
 #include <limits>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -134,6 +135,13 @@ int status_result(uocr_ctx* ctx, unsigned st) {
   if (st & DEV_NORM) return fail(UOCR_ERR_NUMERICAL, "nonfinite numerical input: normalization");
   if (st & DEV_POSITION) return fail(UOCR_ERR_RESOURCE, "resource limit: maximum context exceeded");
   if (st & DEV_CACHE) return fail(UOCR_ERR_SHAPE, "invalid tensor shape: cache must be prefilled");
+  if (st & DEV_KV_RANGE)
+    return fail(UOCR_ERR_NUMERICAL,
+                "nonfinite numerical input: quantised cache value not finite or of magnitude 2^100 and above");
+  if (st & DEV_KV_SLOT)
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: slots past the tokens of the cache");
+  if (st & DEV_TOKEN)
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: token id outside the vocabulary");
   return fail(UOCR_ERR_CUDA, "unknown device status 0x%x", st);
 }
 
@@ -1852,6 +1860,261 @@ int uocr_kv_export(uocr_ctx* ctx, const uocr_kv* kv, size_t seq, float* keys_out
   launch_kv_export(kv->keys, kv->values, kv->layout, static_cast<int>(seq), static_cast<int>(n),
                    keys_out, values_out, ctx->stream);
   return check_launch();
+}
+
+// ---- KV cache held in 4 or 8 bits ---------------------------------------------
+// The states and rules of uocr_kv (LayerCache, src/decoder/cache.rs:3-95) over
+// quantised storage; no counterpart in the reference.
+int uocr_kvq_create(uocr_ctx* ctx, size_t batch, size_t heads, size_t head_dim, size_t window,
+                    size_t max_prefix, int bits, uocr_kvq** out) {
+  if (!ctx || !out) return fail(UOCR_ERR_INVALID, "null argument");
+  *out = nullptr;
+  size_t width;
+  if (!mul_ok(heads, head_dim, &width) || width == 0)
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: cache head dimensions");
+  if (window == 0) return fail(UOCR_ERR_SHAPE, "invalid tensor shape: empty cache window");
+  if (batch == 0 || max_prefix == 0)
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: empty cache batch or prefix");
+  if (bits != 4 && bits != 8)
+    return fail(UOCR_ERR_UNSUPPORTED, "unsupported configuration: cache of %d bits", bits);
+  if (head_dim > static_cast<size_t>(kKvqMaxDim) || heads > 65535 || batch > 65535)
+    return fail(UOCR_ERR_UNSUPPORTED, "unsupported configuration: quantised cache heads or batch");
+  if (max_prefix > (size_t(1) << 30) || window > (size_t(1) << 30) ||
+      max_prefix + window > (size_t(1) << 30))
+    return fail(UOCR_ERR_RESOURCE, "resource limit: cache capacity overflow");
+  auto* kv = new (std::nothrow) uocr_kvq();
+  if (!kv) return fail(UOCR_ERR_RESOURCE, "resource limit: host memory");
+  kv->device = ctx->device;
+  kv->batch = static_cast<int>(batch);
+  kv->width = static_cast<int>(width);
+  kv->window = static_cast<int>(window);
+  kv->max_prefix = static_cast<int>(max_prefix);
+  kv->layout = kvq_layout(static_cast<int>(heads), static_cast<int>(head_dim), bits,
+                          static_cast<long long>(max_prefix + window));
+  // batch, heads < 2^16, tiles <= 2^25, tile < 2^16: below 2^63 after the check
+  size_t n;
+  if (!mul_ok(batch * heads, static_cast<size_t>(kv->layout.tiles), &n) ||
+      !mul_ok(n, static_cast<size_t>(kv->layout.tile), &kv->bytes) || kv->bytes >> 62) {
+    delete kv;
+    return fail(UOCR_ERR_RESOURCE, "resource limit: cache capacity overflow");
+  }
+  try {
+    kv->prefix.assign(batch, 0);
+  } catch (const std::bad_alloc&) {
+    delete kv;
+    return fail(UOCR_ERR_RESOURCE, "resource limit: host memory");
+  }
+  DeviceGuard g(ctx->device);
+  cudaError_t e = cudaMalloc(&kv->data, kv->bytes);
+  if (e == cudaSuccess) e = cudaMalloc(&kv->state, batch * 2 * sizeof(int));
+  if (e == cudaSuccess) e = cudaMemsetAsync(kv->data, 0, kv->bytes, ctx->stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(kv->state, 0, batch * 2 * sizeof(int), ctx->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+  if (e != cudaSuccess) {
+    uocr_kvq_free(kv);
+    cudaGetLastError();
+    return fail(e == cudaErrorMemoryAllocation ? UOCR_ERR_RESOURCE : UOCR_ERR_CUDA,
+                "cache allocation: %s", cudaGetErrorString(e));
+  }
+  *out = kv;
+  return ok();
+}
+
+int uocr_kvq_free(uocr_kvq* kv) {
+  if (!kv) return ok();
+  DeviceGuard g(kv->device);
+  if (kv->data) cudaFree(kv->data);
+  if (kv->state) cudaFree(kv->state);
+  delete kv;
+  return ok();
+}
+
+size_t uocr_kvq_storage_bytes(const uocr_kvq* kv) { return kv ? kv->bytes : 0; }
+
+static int kvq_context(const uocr_ctx* ctx, const uocr_kvq* kv) {
+  if (!ctx || !kv) return fail(UOCR_ERR_INVALID, "null argument");
+  if (ctx->device != kv->device)
+    return fail(UOCR_ERR_INVALID, "the cache lives on device %d, the context on %d", kv->device,
+                ctx->device);
+  return ok();
+}
+
+static int kvq_ready(const uocr_ctx* ctx, const uocr_kvq* kv) {
+  int st = kvq_context(ctx, kv);
+  if (st) return st;
+  for (int p : kv->prefix)
+    if (!p) return fail(UOCR_ERR_SHAPE, "invalid tensor shape: cache must be prefilled");
+  return ok();
+}
+
+// Floats between rows: 0 stands for rows next to each other.
+static int kvq_row_stride(const uocr_kvq* kv, size_t ld, long long* out) {
+  if (ld != 0 && (ld < static_cast<size_t>(kv->width) || ld >> 40))
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: cache row stride");
+  *out = ld ? static_cast<long long>(ld) : kv->width;
+  return ok();
+}
+
+int uocr_kvq_reset(uocr_ctx* ctx, uocr_kvq* kv, size_t seq) {
+  int st = kvq_context(ctx, kv);
+  if (st) return st;
+  if (seq >= static_cast<size_t>(kv->batch))
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: cache sequence");
+  DeviceGuard g(ctx->device);
+  CUDA_TRY(cudaMemsetAsync(kv->state + 2 * seq, 0, 2 * sizeof(int), ctx->stream));
+  kv->prefix[seq] = 0;
+  return ok();
+}
+
+int uocr_kvq_prefill(uocr_ctx* ctx, uocr_kvq* kv, size_t seq, const float* keys_dev, size_t ld_keys,
+                     const float* values_dev, size_t ld_values, size_t tokens) {
+  int st = kvq_context(ctx, kv);
+  if (st) return st;
+  if (seq >= static_cast<size_t>(kv->batch))
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: cache sequence");
+  if (kv->prefix[seq] || tokens == 0)
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: invalid cache prefill");
+  if (tokens > static_cast<size_t>(kv->max_prefix))
+    return fail(UOCR_ERR_RESOURCE, "resource limit: cache capacity overflow");
+  if (!keys_dev || !values_dev) return fail(UOCR_ERR_INVALID, "null argument");
+  long long ld_k, ld_v;
+  if ((st = kvq_row_stride(kv, ld_keys, &ld_k)) || (st = kvq_row_stride(kv, ld_values, &ld_v)))
+    return st;
+  DeviceGuard g(ctx->device);
+  launch_kvq_prefill(kv->data, kv->layout, kv->state, static_cast<int>(seq), keys_dev, ld_k, values_dev,
+                     ld_v, static_cast<int>(tokens), ctx->status_dev, ctx->sms, ctx->stream);
+  if ((st = check_launch())) return st;
+  kv->prefix[seq] = static_cast<int>(tokens);
+  return ok();
+}
+
+int uocr_kvq_push(uocr_ctx* ctx, uocr_kvq* kv, const float* k_dev, size_t ld_k, const float* v_dev,
+                  size_t ld_v) {
+  int st = kvq_ready(ctx, kv);
+  if (st) return st;
+  if (!k_dev || !v_dev) return fail(UOCR_ERR_INVALID, "null argument");
+  long long lk, lv;
+  if ((st = kvq_row_stride(kv, ld_k, &lk)) || (st = kvq_row_stride(kv, ld_v, &lv))) return st;
+  DeviceGuard g(ctx->device);
+  launch_kvq_push(kv->data, kv->layout, kv->state, kv->batch, kv->window, k_dev, lk, v_dev, lv,
+                  ctx->status_dev, ctx->stream);
+  return check_launch();
+}
+
+int uocr_kvq_rope(uocr_ctx* ctx, const uocr_kvq* kv, const uocr_rope* rope, float* q_dev,
+                  float* k_dev) {
+  if (!rope) return fail(UOCR_ERR_INVALID, "null argument");
+  int st = kvq_ready(ctx, kv);
+  if (st) return st;
+  if (rope->head_dim != kv->layout.dim)
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: invalid rotary dimensions or base");
+  if (rope->device != ctx->device || !q_dev) return fail(UOCR_ERR_INVALID, "null argument or rotary table of another device");
+  DeviceGuard g(ctx->device);
+  launch_rope(q_dev, k_dev, kv->width, kv->batch, kv->layout.heads, kv->layout.dim, nullptr, kv->state,
+              rope->table, rope->max_pos, ctx->status_dev, ctx->sms, ctx->stream);
+  return check_launch();
+}
+
+int uocr_kvq_rope_push_qkv(uocr_ctx* ctx, uocr_kvq* kv, const uocr_rope* rope, const float* qkv_dev,
+                           float* q_out_dev) {
+  if (!rope) return fail(UOCR_ERR_INVALID, "null argument");
+  int st = kvq_ready(ctx, kv);
+  if (st) return st;
+  if (rope->head_dim != kv->layout.dim)
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: invalid rotary dimensions or base");
+  if (rope->device != ctx->device || !qkv_dev || !q_out_dev)
+    return fail(UOCR_ERR_INVALID, "null argument or rotary table of another device");
+  DeviceGuard g(ctx->device);
+  launch_kvq_rope_push(kv->data, kv->layout, kv->state, kv->batch, kv->window, qkv_dev, q_out_dev,
+                       rope->table, rope->max_pos, ctx->status_dev, ctx->stream);
+  return check_launch();
+}
+
+int uocr_kvq_attention(uocr_ctx* ctx, const uocr_kvq* kv, const float* q_dev, float* out_dev) {
+  int st = kvq_ready(ctx, kv);
+  if (st) return st;
+  if (!q_dev || !out_dev) return fail(UOCR_ERR_INVALID, "null argument");
+  DeviceGuard g(ctx->device);
+  KvqAttnArgs a{};
+  a.data = kv->data;
+  a.layout = kv->layout;
+  a.state = kv->state;
+  a.window = kv->window;
+  a.q = q_dev;
+  a.out = out_dev;
+  a.scale = 1.0f / std::sqrt(static_cast<float>(kv->layout.dim));
+  a.status = ctx->status_dev;
+  a.sms = ctx->sms;
+  const cudaError_t e = launch_kvq_attention(a, kv->batch, ctx->stream);
+  if (e != cudaSuccess) return fail(UOCR_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
+  return ok();
+}
+
+int uocr_kvq_state(uocr_ctx* ctx, const uocr_kvq* kv, size_t seq, size_t* tokens, size_t* position) {
+  int st = kvq_context(ctx, kv);
+  if (st) return st;
+  if (seq >= static_cast<size_t>(kv->batch))
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: cache sequence");
+  DeviceGuard g(ctx->device);
+  int h[2];
+  CUDA_TRY(cudaMemcpyAsync(h, kv->state + 2 * seq, sizeof h, cudaMemcpyDeviceToHost, ctx->stream));
+  CUDA_TRY(cudaStreamSynchronize(ctx->stream));
+  const size_t gen = static_cast<size_t>(h[1]), win = static_cast<size_t>(kv->window);
+  if (tokens) *tokens = static_cast<size_t>(h[0]) + (gen < win ? gen : win);
+  if (position) *position = static_cast<size_t>(h[0]) + gen;
+  return take_device_status(ctx);
+}
+
+int uocr_kvq_read(uocr_ctx* ctx, const uocr_kvq* kv, size_t seq, size_t first, size_t count,
+                  float* keys_out_dev, float* values_out_dev) {
+  int st = kvq_context(ctx, kv);
+  if (st) return st;
+  if (seq >= static_cast<size_t>(kv->batch))
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: cache sequence");
+  const size_t slots = static_cast<size_t>(kv->prefix[seq]) + (kv->prefix[seq] ? kv->window : 0);
+  if (first > slots || count > slots - first)
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: slots past the tokens of the cache");
+  if (count == 0) return ok();
+  if (!keys_out_dev || !values_out_dev) return fail(UOCR_ERR_INVALID, "null argument");
+  DeviceGuard g(ctx->device);
+  launch_kvq_read(kv->data, kv->layout, kv->state, kv->window, static_cast<int>(seq),
+                  static_cast<long long>(first), static_cast<long long>(count), keys_out_dev,
+                  values_out_dev, ctx->status_dev, ctx->sms, ctx->stream);
+  return check_launch();
+}
+
+// ---- what the logits say ------------------------------------------------------
+int uocr_token_logprobs(uocr_ctx* ctx, const float* logits_dev, size_t rows, size_t vocab, size_t ld,
+                        const int64_t* tokens_dev, size_t top_k, float* logprob_dev,
+                        float* entropy_dev, int64_t* top_ids_dev, float* top_logprobs_dev) {
+  if (!ctx) return fail(UOCR_ERR_INVALID, "null context");
+  if (vocab == 0 || (ld != 0 && ld < vocab))
+    return fail(UOCR_ERR_SHAPE, "invalid tensor shape: logits row");
+  if (top_k > vocab) return fail(UOCR_ERR_SHAPE, "invalid tensor shape: more alternatives than logits");
+  if (top_k > static_cast<size_t>(kLogprobMaxTop))
+    return fail(UOCR_ERR_UNSUPPORTED, "unsupported configuration: more than %d alternatives", kLogprobMaxTop);
+  if (!fits_int(vocab) || !fits_int(rows) || ld >> 40)
+    return fail(UOCR_ERR_UNSUPPORTED, "unsupported configuration: logits extent above 2^31");
+  if ((tokens_dev == nullptr) != (logprob_dev == nullptr))
+    return fail(UOCR_ERR_INVALID, "token ids and their log probabilities come together");
+  if (rows == 0) return ok();
+  if (!logits_dev || (top_k && (!top_ids_dev || !top_logprobs_dev)))
+    return fail(UOCR_ERR_INVALID, "null argument");
+  DeviceGuard g(ctx->device);
+  LogprobArgs a{};
+  a.logits = logits_dev;
+  a.ld = static_cast<long long>(ld ? ld : vocab);
+  a.vocab = static_cast<int>(vocab);
+  a.top_k = static_cast<int>(top_k);
+  a.tokens = reinterpret_cast<const long long*>(tokens_dev);
+  a.logprob = logprob_dev;
+  a.entropy = entropy_dev;
+  a.top_ids = reinterpret_cast<long long*>(top_ids_dev);
+  a.top_logprobs = top_logprobs_dev;
+  a.status = ctx->status_dev;
+  const cudaError_t e = launch_token_logprobs(a, static_cast<int>(rows), ctx->sms, ctx->stream);
+  if (e != cudaSuccess) return fail(UOCR_ERR_CUDA, "log probabilities launch: %s", cudaGetErrorString(e));
+  return ok();
 }
 
 }  // extern "C"

@@ -33,6 +33,9 @@ enum DevStatus : unsigned {
   DEV_NORM = 1u << 8,           // normalization row or weight held NaN or Inf
   DEV_POSITION = 1u << 9,       // rotary position outside the table (context exceeded)
   DEV_CACHE = 1u << 10,         // KV cache used before its prefill
+  DEV_KV_RANGE = 1u << 11,      // value for a quantised cache not finite or too large
+  DEV_KV_SLOT = 1u << 12,       // slots read that a cache does not hold
+  DEV_TOKEN = 1u << 13,         // token id outside the vocabulary
 };
 
 __device__ __forceinline__ void flag(unsigned* status, unsigned bits) {

@@ -100,3 +100,15 @@ struct uocr_kv {
   float* scores = nullptr;  // split attention scratch [batch][heads][cap] (tiled layout)
   int split = 0;            // attention form: 0 by batch size, 1 one CTA per head, 2 split
 };
+
+// KV cache of `batch` sequences held in `layout.bits` bits: tiles per
+// (sequence, head), device state {prefix, generated} as uocr_kv.
+struct uocr_kvq {
+  int device = 0;
+  int batch = 0, width = 0, window = 0, max_prefix = 0;
+  uocr::KvqLayout layout{};
+  size_t bytes = 0;
+  unsigned char* data = nullptr;
+  int* state = nullptr;
+  std::vector<int> prefix;  // host mirror (0: not prefilled)
+};

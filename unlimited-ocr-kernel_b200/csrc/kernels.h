@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "kv_quant.cuh"
+
 namespace uocr {
 
 // Device view of one q8-block32 matrix.
@@ -339,6 +341,54 @@ cudaError_t launch_attention_prefill(const AttnMaps& m, const AttnArgs& a, cudaS
 cudaError_t launch_attention_split(const AttnArgs& a, int batch, int max_tokens, cudaStream_t st);
 cudaError_t launch_attention_decode_tma(const AttnMaps& m, const AttnArgs& a, int batch,
                                         cudaStream_t st);
+// kv_quant.cu — KV cache in 4 or 8 bits (layout: kv_quant.cuh).  Rows of k and
+// v are ld_k / ld_v floats apart, heads of dim floats next to each other.
+// Rows 0..tokens-1 into slots 0.. of sequence seq, whose state becomes
+// {tokens, 0}.
+void launch_kvq_prefill(unsigned char* data, const KvqLayout& L, int* state, int seq, const float* k,
+                        long long ld_k, const float* v, long long ld_v, int tokens,
+                        unsigned* status, int sms, cudaStream_t st);
+// Row b into the next slot of every sequence b.
+void launch_kvq_push(unsigned char* data, const KvqLayout& L, int* state, int batch, int window,
+                     const float* k, long long ld_k, const float* v, long long ld_v,
+                     unsigned* status, cudaStream_t st);
+// Rope of q and k plus the push, from fused rows [q | k | v].
+void launch_kvq_rope_push(unsigned char* data, const KvqLayout& L, int* state, int batch, int window,
+                          const float* qkv, float* q_out, const float2* table, int max_pos,
+                          unsigned* status, cudaStream_t st);
+// Slots [first, first + count) of sequence seq as rows of heads * dim floats.
+void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* state, int window,
+                     int seq, long long first, long long count, float* k, float* v, unsigned* status,
+                     int sms, cudaStream_t st);
+struct KvqAttnArgs {
+  const unsigned char* data;
+  KvqLayout layout;
+  const int* state;  // {prefix, generated} per sequence
+  int window;
+  const float* q;    // [batch][heads * dim]
+  float* out;        // the same
+  float scale;       // 1 / sqrt(dim)
+  unsigned* status;
+  int sms;
+};
+cudaError_t launch_kvq_attention(const KvqAttnArgs& a, int batch, cudaStream_t st);
+
+// logprobs.cu — per row of logits: log probability of the given token,
+// entropy, top alternatives.
+struct LogprobArgs {
+  const float* logits;
+  long long ld;              // floats between rows
+  int vocab, top_k;
+  const long long* tokens;   // [rows], or null
+  float* logprob;            // [rows], with tokens
+  float* entropy;            // [rows], or null
+  long long* top_ids;        // [rows][top_k], or null when top_k is 0
+  float* top_logprobs;       // the same
+  unsigned* status;
+};
+constexpr int kLogprobMaxTop = 32;
+cudaError_t launch_token_logprobs(const LogprobArgs& a, int rows, int sms, cudaStream_t st);
+
 // rope_table.cpp — host: the reference's cos/sin of every (position, pair).
 void build_rope_table(int dim, float theta, int max_pos, float* cos_sin /* [max_pos][dim/2][2] */);
 

@@ -96,6 +96,18 @@ SIGNATURES = {
     "uocr_kv_rope_push_qkv": (I, [P, P, P, P, P]),
     "uocr_kv_state": (I, [P, P, S, ctypes.POINTER(S), ctypes.POINTER(S)]),
     "uocr_kv_export": (I, [P, P, S, P, P, ctypes.POINTER(S)]),
+    "uocr_kvq_create": (I, [P, S, S, S, S, S, I, PP]),
+    "uocr_kvq_free": (I, [P]),
+    "uocr_kvq_storage_bytes": (S, [P]),
+    "uocr_kvq_reset": (I, [P, P, S]),
+    "uocr_kvq_prefill": (I, [P, P, S, P, S, P, S, S]),
+    "uocr_kvq_push": (I, [P, P, P, S, P, S]),
+    "uocr_kvq_rope": (I, [P, P, P, P, P]),
+    "uocr_kvq_rope_push_qkv": (I, [P, P, P, P, P]),
+    "uocr_kvq_attention": (I, [P, P, P, P]),
+    "uocr_kvq_state": (I, [P, P, S, ctypes.POINTER(S), ctypes.POINTER(S)]),
+    "uocr_kvq_read": (I, [P, P, S, S, S, P, P]),
+    "uocr_token_logprobs": (I, [P, P, S, S, S, P, S, P, P, P, P]),
     "uocr_overlay_check": (I, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(S),
                                ctypes.POINTER(S)]),
     "uocr_overlay_load": (I, [P, ctypes.c_char_p, ctypes.c_char_p, PP]),

@@ -24,12 +24,13 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, NamedTuple, Optional
 
 import numpy as np
 
 from . import (GpuContext, Int8Matrix, MoeLayer, QuantizationMode, _check, _tptr, lib)
-from .attention import KvCache, Rope, add_rms_norm_device, rms_norm_device
+from .attention import (KvCache, QuantizedKvCache, Rope, add_rms_norm_device,
+                        attention_prefill_device, rms_norm_device)
 
 
 @dataclass
@@ -188,13 +189,18 @@ class Decoder:
 
 
 class DecodeState:
-    """Per-layer KV caches (LayerCache for every sequence) and the rotary table."""
+    """Per-layer KV caches (LayerCache for every sequence) and the rotary
+    table.  ``kv_bits`` 32 holds them in FP32 (the reference's results), 8 or 4
+    in that many bits (``QuantizedKvCache``: a prefill attends to its own FP32
+    rows, the decode steps after it to what the cache holds)."""
 
-    def __init__(self, decoder: Decoder, batch: int, max_prefix: int):
+    def __init__(self, decoder: Decoder, batch: int, max_prefix: int, kv_bits: int = 32):
         cfg = decoder.cfg
         self.batch = batch
         self.max_prefix = max_prefix
-        self.caches = [KvCache(decoder.ctx, batch, cfg.heads, cfg.head_dim, cfg.window, max_prefix)
+        self.kv_bits = kv_bits
+        shape = (decoder.ctx, batch, cfg.heads, cfg.head_dim, cfg.window, max_prefix)
+        self.caches = [KvCache(*shape) if kv_bits == 32 else QuantizedKvCache(*shape, kv_bits)
                        for _ in range(cfg.layers)]
         self.rope = Rope(decoder.ctx, cfg.head_dim, cfg.theta, cfg.max_positions)
 
@@ -284,7 +290,10 @@ def prefill(decoder: Decoder, state: DecodeState, embeddings_t, mode: int = 0, s
         q, k, v = (qkv[:, i * H:(i + 1) * H].contiguous() for i in range(3))
         state.rope.apply(q, k, positions)
         cache.prefill(seq, k, v)
-        a = cache.attention_prefill(seq, q)
+        if isinstance(cache, QuantizedKvCache):  # the prompt attends to its own FP32 rows
+            a = attention_prefill_device(ctx, q, k, v, cfg.heads)
+        else:
+            a = cache.attention_prefill(seq, q)
         r = layer.o.linear_device(a, dynamic=dyn)
         n = add_rms_norm_device(ctx, r, x, layer.post_norm, cfg.eps, sum_t=r)  # r += x
         if layer.moe is not None:
@@ -304,6 +313,54 @@ def logits_checksum_device(ctx: GpuContext, logits_t, acc_t):
     """acc_t (int64 [1], device) += the bit patterns of logits_t as u64,
     wrapping (the fixed-work benchmark's checksum, uocr_bits_checksum)."""
     _check(lib().uocr_bits_checksum(ctx.handle, _p(logits_t), logits_t.numel(), _p(acc_t)))
+
+
+class TokenLogprobs(NamedTuple):
+    """What rows of logits say: ``logprob`` [rows] of the given tokens (None
+    without tokens), ``entropy`` [rows], ``top_ids`` (int64) and
+    ``top_logprobs`` [rows x top_k]."""
+    logprob: Optional[object]
+    entropy: object
+    top_ids: object
+    top_logprobs: object
+
+
+def token_logprobs_device(ctx: GpuContext, logits_t, tokens_t=None, top_k: int = 0) -> TokenLogprobs:
+    """Log probabilities (natural) of tokens_t (int64 [rows], negative: none)
+    under the rows of logits_t [rows x vocab] (FP32, rows may lie apart), the
+    rows' entropies and top_k most probable tokens, equal ones by the lower id
+    (uocr_token_logprobs).  -inf bans a token.  Asynchronous."""
+    import torch
+
+    from . import OcrError
+    if logits_t.dim() != 2 or logits_t.dtype != torch.float32 or not logits_t.is_cuda:
+        raise OcrError(4, "invalid tensor shape: logits: FP32 CUDA rows [rows x vocab] expected")
+    rows, vocab = logits_t.shape
+    if (vocab > 1 and logits_t.stride(1) != 1) or (rows > 1 and logits_t.stride(0) < vocab):
+        raise OcrError(4, "invalid tensor shape: logits: rows of adjacent floats expected")
+    if tokens_t is not None and (tokens_t.dtype != torch.int64 or not tokens_t.is_cuda
+                                 or tokens_t.shape != (rows,) or not tokens_t.is_contiguous()):
+        raise OcrError(4, "invalid tensor shape: tokens: contiguous int64 CUDA [rows] expected")
+    if top_k < 0:
+        raise OcrError(4, "invalid tensor shape: top_k must not be negative")
+    new = lambda *shape, **kw: torch.empty(shape, device=logits_t.device, **kw)  # noqa: E731
+    out = TokenLogprobs(new(rows) if tokens_t is not None else None, new(rows),
+                        new(rows, top_k, dtype=torch.int64), new(rows, top_k))
+    opt = lambda t: _p(t) if t is not None and t.numel() else None  # noqa: E731
+    _check(lib().uocr_token_logprobs(ctx.handle, _p(logits_t), rows, vocab,
+                                     logits_t.stride(0) if rows > 1 else vocab, opt(tokens_t),
+                                     top_k, opt(out.logprob), _p(out.entropy), opt(out.top_ids),
+                                     opt(out.top_logprobs)))
+    return out
+
+
+def score_step(decoder: Decoder, state: DecodeState, tokens_t, next_t, mode: int = 0, top_k: int = 0,
+               logits_t=None, experts=None) -> TokenLogprobs:
+    """One teacher-forced decode step: ``decode_step`` of tokens_t, then the log
+    probabilities of next_t (int64 [batch], the tokens that follow) under its
+    logits, their entropies and top_k alternatives.  Asynchronous."""
+    logits = decode_step(decoder, state, tokens_t, mode, logits_t, experts)
+    return token_logprobs_device(decoder.ctx, logits, next_t, top_k)
 
 
 # ---- loading a checkpoint with its INT8 overlay -------------------------------
@@ -532,4 +589,5 @@ def load_decoder(ctx: GpuContext, directory, overlay_path,
 
 
 __all__ = ["DecoderConfig", "Decoder", "DecoderLayer", "DecodeState", "decode_step",
+           "TokenLogprobs", "token_logprobs_device", "score_step",
            "linear_bf16_device", "feed_forward_device", "config_from_json", "load_decoder"]
