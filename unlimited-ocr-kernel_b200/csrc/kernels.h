@@ -370,8 +370,9 @@ struct KvqAttnArgs {
   float scale;       // 1 / sqrt(dim)
   unsigned* status;
   int sms;
+  int splits;        // CTAs per (head, sequence): set by the launcher
 };
-cudaError_t launch_kvq_attention(const KvqAttnArgs& a, int batch, cudaStream_t st);
+cudaError_t launch_kvq_attention(KvqAttnArgs a, int batch, cudaStream_t st);
 
 // logprobs.cu — per row of logits: log probability of the given token,
 // entropy, top alternatives.
