@@ -1906,9 +1906,12 @@ int uocr_kvq_create(uocr_ctx* ctx, size_t batch, size_t heads, size_t head_dim, 
   }
   DeviceGuard g(ctx->device);
   cudaError_t e = cudaMalloc(&kv->data, kv->bytes);
-  if (e == cudaSuccess) e = cudaMalloc(&kv->state, batch * 2 * sizeof(int));
+  const size_t ints = batch * 2 + kvq_units(ctx->sms);
+  if (e == cudaSuccess) e = cudaMalloc(&kv->state, ints * sizeof(int));
+  if (e == cudaSuccess)
+    e = cudaMalloc(&kv->partial, kvq_units(ctx->sms) * (head_dim + 2) * sizeof(float));
   if (e == cudaSuccess) e = cudaMemsetAsync(kv->data, 0, kv->bytes, ctx->stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(kv->state, 0, batch * 2 * sizeof(int), ctx->stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(kv->state, 0, ints * sizeof(int), ctx->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
   if (e != cudaSuccess) {
     uocr_kvq_free(kv);
@@ -1925,6 +1928,7 @@ int uocr_kvq_free(uocr_kvq* kv) {
   DeviceGuard g(kv->device);
   if (kv->data) cudaFree(kv->data);
   if (kv->state) cudaFree(kv->state);
+  if (kv->partial) cudaFree(kv->partial);
   delete kv;
   return ok();
 }
@@ -1982,7 +1986,7 @@ int uocr_kvq_prefill(uocr_ctx* ctx, uocr_kvq* kv, size_t seq, const float* keys_
     return st;
   DeviceGuard g(ctx->device);
   launch_kvq_prefill(kv->data, kv->layout, kv->state, static_cast<int>(seq), keys_dev, ld_k, values_dev,
-                     ld_v, static_cast<int>(tokens), ctx->status_dev, ctx->sms, ctx->stream);
+                     ld_v, static_cast<int>(tokens), ctx->status_dev, ctx->stream);
   if ((st = check_launch())) return st;
   kv->prefix[seq] = static_cast<int>(tokens);
   return ok();
@@ -2045,6 +2049,8 @@ int uocr_kvq_attention(uocr_ctx* ctx, const uocr_kvq* kv, const float* q_dev, fl
   a.scale = 1.0f / std::sqrt(static_cast<float>(kv->layout.dim));
   a.status = ctx->status_dev;
   a.sms = ctx->sms;
+  a.partial = kv->partial;
+  a.tickets = kv->state + 2 * kv->batch;
   const cudaError_t e = launch_kvq_attention(a, kv->batch, ctx->stream);
   if (e != cudaSuccess) return fail(UOCR_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
   return ok();
@@ -2079,7 +2085,7 @@ int uocr_kvq_read(uocr_ctx* ctx, const uocr_kvq* kv, size_t seq, size_t first, s
   DeviceGuard g(ctx->device);
   launch_kvq_read(kv->data, kv->layout, kv->state, kv->window, static_cast<int>(seq),
                   static_cast<long long>(first), static_cast<long long>(count), keys_out_dev,
-                  values_out_dev, ctx->status_dev, ctx->sms, ctx->stream);
+                  values_out_dev, ctx->status_dev, ctx->stream);
   return check_launch();
 }
 

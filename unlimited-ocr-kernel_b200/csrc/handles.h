@@ -109,6 +109,7 @@ struct uocr_kvq {
   uocr::KvqLayout layout{};
   size_t bytes = 0;
   unsigned char* data = nullptr;
-  int* state = nullptr;
+  int* state = nullptr;     // [batch][2], then the attention's tickets
+  float* partial = nullptr; // the attention's parts (KvqAttnArgs)
   std::vector<int> prefix;  // host mirror (0: not prefilled)
 };

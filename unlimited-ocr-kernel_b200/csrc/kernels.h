@@ -347,7 +347,7 @@ cudaError_t launch_attention_decode_tma(const AttnMaps& m, const AttnArgs& a, in
 // {tokens, 0}.
 void launch_kvq_prefill(unsigned char* data, const KvqLayout& L, int* state, int seq, const float* k,
                         long long ld_k, const float* v, long long ld_v, int tokens,
-                        unsigned* status, int sms, cudaStream_t st);
+                        unsigned* status, cudaStream_t st);
 // Row b into the next slot of every sequence b.
 void launch_kvq_push(unsigned char* data, const KvqLayout& L, int* state, int batch, int window,
                      const float* k, long long ld_k, const float* v, long long ld_v,
@@ -359,7 +359,7 @@ void launch_kvq_rope_push(unsigned char* data, const KvqLayout& L, int* state, i
 // Slots [first, first + count) of sequence seq as rows of heads * dim floats.
 void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* state, int window,
                      int seq, long long first, long long count, float* k, float* v, unsigned* status,
-                     int sms, cudaStream_t st);
+                     cudaStream_t st);
 struct KvqAttnArgs {
   const unsigned char* data;
   KvqLayout layout;
@@ -370,9 +370,19 @@ struct KvqAttnArgs {
   float scale;       // 1 / sqrt(dim)
   unsigned* status;
   int sms;
-  int splits;        // CTAs per (head, sequence): set by the launcher
+  // heads spread over several clusters of CTAs: a part's {max, sum, values} per
+  // cluster and a ticket per (sequence, head), zero between launches
+  float* partial;
+  int* tickets;
+  int splits, parts;  // CTAs per cluster, clusters per head: set by the launcher
 };
-cudaError_t launch_kvq_attention(KvqAttnArgs a, int batch, cudaStream_t st);
+constexpr int kKvqMaxParts = 16;
+// Heads are spread over several clusters (of two CTAs at least) only while
+// their CTAs are resident at once, counted as eight per SM at most: so `tickets`
+// has kvq_units ints, and `partial` kvq_units rows of dim + 2 floats.
+constexpr int kKvqCtasPerSm = 8;
+inline size_t kvq_units(int sms) { return static_cast<size_t>(sms) * kKvqCtasPerSm / 2; }
+cudaError_t launch_kvq_attention(const KvqAttnArgs& a, int batch, cudaStream_t st);
 
 // logprobs.cu — per row of logits: log probability of the given token,
 // entropy, top alternatives.

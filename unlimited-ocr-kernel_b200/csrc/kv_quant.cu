@@ -20,12 +20,6 @@ namespace uocr {
 __device__ __forceinline__ float bf16_low(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
-// Values of larger magnitude are refused, so that no difference, step or
-// product above overflows.
-__device__ __forceinline__ bool kvq_in_range(float x) {
-  return fabsf(x) < 1.2676506e30f;  // 2^100; false for NaN
-}
-
 // Step and least value of a group from its extremes, packed (s low, m high).
 __device__ __forceinline__ uint32_t kvq_params(float lo, float hi, double inv_levels, double levels,
                                                float* s_out, float* m_out) {
@@ -45,58 +39,63 @@ __device__ __forceinline__ uint32_t kvq_params(float lo, float hi, double inv_le
   return (sb >> 16) | mb;
 }
 
-// Code of x: in float, and in double where the float quotient is too near a
-// border between two codes (or the step too small) to decide.  The float
-// quotient is off by at most 3 roundings of 2^-24, so by 5e-5 at 255.
-__device__ __forceinline__ int kvq_code(float x, float m, float s, float inv_s, int levels) {
-  const float t = __fmul_rn(__fsub_rn(x, m), inv_s);
-  const float r = rintf(t);
-  int c = static_cast<int>(r);
-  if (!(fabsf(t - r) < 0.4999f) || s < 1e-30f)
-    c = s > 0.0f ? __double2int_rn(__ddiv_rn(__dsub_rn(static_cast<double>(x), static_cast<double>(m)),
-                                             static_cast<double>(s)))
-                 : 0;
-  return min(max(c, 0), levels);
+__device__ __forceinline__ float rcp_fast(float x) {  // 1 ulp; subnormals count as 0
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// One head's row of a key (VALUE false) or value into token t of a tile, by
-// one warp, lane = dim of the group: x(d) gives the row.
-template <bool VALUE, class Row>
-__device__ __forceinline__ void kvq_write_row(unsigned char* tile, const KvqLayout& L, int t, Row x,
-                                              unsigned* status) {
-  const int lane = threadIdx.x & 31;
-  const int levels = (1 << L.bits) - 1;
-  const double dl = levels, inv = __ddiv_rn(1.0, dl);
-  unsigned char* codes = tile + (VALUE ? L.half : 0);
-  for (int grp = 0; grp < L.groups; ++grp) {
-    const int d = grp * kKvqGroup + lane;
-    const bool in = d < L.dim;
-    const float v = in ? x(d) : 0.0f;
-    const bool bad = __any_sync(0xffffffffu, in && !kvq_in_range(v));
-    float lo = in ? v : INFINITY, hi = in ? v : -INFINITY;
+// Codes of four values as the bytes of a word: in float, rounded by adding
+// 1.5 2^23 (whose last place is 1), and again in double where a quotient is too
+// near a border between two codes, or the step too small, to decide.  The float
+// quotient is off by four roundings of 2^-24 at most, so by 6e-5 at 255.
+__device__ __forceinline__ uint32_t kvq_codes4(const float (&x)[4], float m, float s, float inv_s,
+                                               int levels) {
+  uint32_t c[4];
+  float worst = 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    float s, m;
-    uint32_t word = kvq_params(lo, hi, inv, dl, &s, &m);
-    int c = in ? kvq_code(v, m, s, __fdiv_rn(1.0f, s), levels) : 0;
-    if (bad) {  // the group reads as NaN
-      word = 0x7FC00000u;
-      c = 0;
-      if (lane == 0) flag(status, DEV_KV_RANGE);
-    }
-    const int at = VALUE ? kvq_value_byte(t, d, L.bits) : kvq_key_byte(t, d, L.bits);
-    if (L.bits == 4) {
-      const int up = VALUE ? 8 : 16;  // the dim whose code is the high nibble
-      const int high = __shfl_xor_sync(0xffffffffu, c, up);
-      if (!(lane & up)) codes[at] = static_cast<unsigned char>(c | (high << 4));
-    } else {
-      codes[at] = static_cast<unsigned char>(c);
-    }
-    if (lane == 0) *reinterpret_cast<uint32_t*>(codes + L.codes + kvq_param_byte(t, grp)) = word;
+  for (int i = 0; i < 4; ++i) {
+    const float t = __fmul_rn(__fsub_rn(x[i], m), inv_s);
+    const float r = __fadd_rn(t, 12582912.0f);
+    c[i] = __float_as_uint(r);
+    const float off = fabsf(__fsub_rn(t, __fsub_rn(r, 12582912.0f)));
+    worst = off < 0.4999f ? worst : 1.0f;  // (1 for NaN as well)
   }
+  if (worst != 0.0f || s < 1e-30f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int v = 0;
+      if (s > 0.0f)
+        v = __double2int_rn(__ddiv_rn(__dsub_rn(static_cast<double>(x[i]), static_cast<double>(m)),
+                                      static_cast<double>(s)));
+      c[i] = static_cast<uint32_t>(min(max(v, 0), levels));
+    }
+  }
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+
+// Four values of a row from dim d (a multiple of 4); zeros past the row's end.
+template <bool VEC>
+__device__ __forceinline__ void kvq_load4(const float* row, int d, int dim, float (&x)[4]) {
+  if (VEC) {
+    const float4 v = d < dim ? __ldg(reinterpret_cast<const float4*>(row + d))
+                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    x[0] = v.x;
+    x[1] = v.y;
+    x[2] = v.z;
+    x[3] = v.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = d + i < dim ? __ldg(row + d + i) : 0.0f;
+  }
+}
+
+// Whether one of four values is not below 2^100 in magnitude.
+__device__ __forceinline__ bool kvq_refused(const float (&x)[4]) {
+  uint32_t u = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u = max(u, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  return u >= 0x71800000u;
 }
 
 __device__ __forceinline__ unsigned char* kvq_tile(unsigned char* data, const KvqLayout& L, int seq,
@@ -104,44 +103,152 @@ __device__ __forceinline__ unsigned char* kvq_tile(unsigned char* data, const Kv
   return data + ((static_cast<long long>(seq) * L.heads + head) * L.tiles + (slot >> 5)) * L.tile;
 }
 
-// A prompt's rows: one warp per (token, head).
+// ---- a prompt's rows ------------------------------------------------------------
+// One CTA per (tile, head), one warp per four neighbouring tokens, so that the
+// bytes of a value word (four tokens of one dim) meet in one lane.  Eight lanes
+// share a group, four dims each; four groups at a time.  The extremes of four
+// tokens are eight values over eight lanes: halving what a lane keeps at every
+// exchange takes 7 shuffles instead of 24 and leaves the extremes of token u in
+// the lanes u and u + 4 of the eight, which then find its parameters once.
+template <int BITS, bool VEC>
 __global__ void __launch_bounds__(256)
     kvq_prefill_kernel(unsigned char* data, const KvqLayout L, int* state, int seq,
                        const float* __restrict__ k, long long ld_k, const float* __restrict__ v,
                        long long ld_v, int tokens, unsigned* status) {
+  extern __shared__ __align__(16) unsigned char kvq_stage[];
+  constexpr int levels = (1 << BITS) - 1;
+  const int h = blockIdx.x % L.heads, tile = blockIdx.x / L.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     state[2 * seq] = tokens;
     state[2 * seq + 1] = 0;
   }
-  const long long rows = static_cast<long long>(tokens) * L.heads;
-  for (long long r = blockIdx.x * 8LL + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8LL) {
-    const int t = static_cast<int>(r / L.heads), h = static_cast<int>(r % L.heads);
-    unsigned char* tile = kvq_tile(data, L, seq, h, t);
-    const float* kr = k + t * ld_k + static_cast<long long>(h) * L.dim;
-    const float* vr = v + t * ld_v + static_cast<long long>(h) * L.dim;
-    kvq_write_row<false>(tile, L, t & 31, [&](int d) { return kr[d]; }, status);
-    kvq_write_row<true>(tile, L, t & 31, [&](int d) { return vr[d]; }, status);
+  const int t0 = tile * 32 + warp * 4;  // this warp's tokens: t0 .. t0 + 3
+  const int half = warp >> 2, j = warp & 3;
+  for (int q = 0; q < (L.groups + 3) / 4; ++q) {
+    const int grp = q * 4 + (lane >> 3), d0 = grp * 32 + l8 * 4;
+    const bool real = grp < L.groups;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const float* rows = (part ? v : k) + static_cast<long long>(h) * L.dim;
+      const long long ld = part ? ld_v : ld_k;
+      float x[4][4];
+      bool refused = false;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (t0 + u < tokens) {
+          kvq_load4<VEC>(rows + (t0 + u) * ld, d0, L.dim, x[u]);
+        } else {
+          x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
+        }
+      }
+      // the largest x and the largest -x of each token, over this lane's dims
+      float a[4], b[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        refused |= kvq_refused(x[u]);
+        a[u] = b[u] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (d0 + i < L.dim) {
+            a[u] = fmaxf(a[u], x[u][i]);
+            b[u] = fmaxf(b[u], -x[u][i]);
+          }
+      }
+      const bool h4 = l8 & 4, h2 = l8 & 2, h1 = l8 & 1;
+      float e[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        e[u] = fmaxf(h4 ? b[u] : a[u], __shfl_xor_sync(0xffffffffu, h4 ? a[u] : b[u], 4));
+      const float e0 = fmaxf(h2 ? e[2] : e[0], __shfl_xor_sync(0xffffffffu, h2 ? e[0] : e[2], 2));
+      const float e1 = fmaxf(h2 ? e[3] : e[1], __shfl_xor_sync(0xffffffffu, h2 ? e[1] : e[3], 2));
+      const float mine = fmaxf(h1 ? e1 : e0, __shfl_xor_sync(0xffffffffu, h1 ? e0 : e1, 1));
+      const float other = __shfl_xor_sync(0xffffffffu, mine, 4);
+      float s, m;
+      uint32_t word = kvq_params(-(h4 ? mine : other), h4 ? other : mine, 1.0 / levels, levels, &s, &m);
+      const float inv_s = rcp_fast(s);
+      // a group that holds a refused value reads as NaN
+      unsigned lost = 0;
+      if (__any_sync(0xffffffffu, refused)) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if ((__ballot_sync(0xffffffffu, kvq_refused(x[u])) >> (lane & 24)) & 0xFFu) lost |= 1u << u;
+        if (lost) flag(status, DEV_KV_RANGE);
+        if ((lost >> (l8 & 3)) & 1) word = 0x7FC00000u;
+      }
+      unsigned char* codes = kvq_stage + part * L.half;
+      if (real && l8 < 4)
+        *reinterpret_cast<uint32_t*>(codes + L.codes + kvq_param_byte(warp * 4 + l8, grp)) = word;
+      uint32_t c[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int from = (lane & 24) + u;
+        c[u] = kvq_codes4(x[u], __shfl_sync(0xffffffffu, m, from), __shfl_sync(0xffffffffu, s, from),
+                          __shfl_sync(0xffffffffu, inv_s, from), levels);
+        if ((lost >> u) & 1) c[u] = 0;
+        if (d0 + 3 >= L.dim) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (d0 + i >= L.dim) c[u] &= ~(0xFFu << (8 * i));
+        }
+      }
+      if (part == 0) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (BITS == 4) c[u] |= __shfl_xor_sync(0xffffffffu, c[u], 4) << 4;
+          if (real && (BITS == 8 || !h4))
+            *reinterpret_cast<uint32_t*>(codes + kvq_key_byte(warp * 4 + u, d0, BITS)) = c[u];
+        }
+      } else {
+        // bytes: token u of dim i; as words: dim i of the four tokens
+        const uint32_t lo = __byte_perm(c[0], c[1], 0x5140), hi = __byte_perm(c[0], c[1], 0x7362);
+        const uint32_t lo2 = __byte_perm(c[2], c[3], 0x5140), hi2 = __byte_perm(c[2], c[3], 0x7362);
+        uint32_t w[4] = {__byte_perm(lo, lo2, 0x5410), __byte_perm(lo, lo2, 0x7632),
+                         __byte_perm(hi, hi2, 0x5410), __byte_perm(hi, hi2, 0x7632)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (BITS == 4) w[i] |= __shfl_xor_sync(0xffffffffu, w[i], 2) << 4;
+          if (real && (BITS == 8 || !h2))
+            *reinterpret_cast<uint32_t*>(codes + kvq_value_byte(half * 16 + j * 4, d0 + i, BITS)) = w[i];
+        }
+      }
+    }
   }
+  __syncthreads();
+  // (slots past the prompt's end in its last tile get zeros: nothing is in them)
+  uint4* out = reinterpret_cast<uint4*>(kvq_tile(data, L, seq, h, tile * 32LL));
+  const uint4* in = reinterpret_cast<const uint4*>(kvq_stage);
+  for (int i = threadIdx.x; i < L.tile / 16; i += 256) out[i] = in[i];
+}
+
+// Rows that four floats at a time can be read from (or written to).
+static bool kvq_vec(const KvqLayout& L, const void* k, long long ld_k, const void* v, long long ld_v) {
+  return L.dim % 4 == 0 && ld_k % 4 == 0 && ld_v % 4 == 0 && reinterpret_cast<uintptr_t>(k) % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(v) % 16 == 0;
 }
 
 void launch_kvq_prefill(unsigned char* data, const KvqLayout& L, int* state, int seq, const float* k,
                         long long ld_k, const float* v, long long ld_v, int tokens,
-                        unsigned* status, int sms, cudaStream_t st) {
-  const long long rows = static_cast<long long>(tokens) * L.heads;
-  const long long blocks = (rows + 7) / 8, most = 16LL * sms;
-  kvq_prefill_kernel<<<static_cast<int>(blocks < most ? blocks : most), 256, 0, st>>>(
-      data, L, state, seq, k, ld_k, v, ld_v, tokens, status);
+                        unsigned* status, cudaStream_t st) {
+  const unsigned blocks = static_cast<unsigned>((tokens + 31) / 32) * L.heads;
+  const bool vec = kvq_vec(L, k, ld_k, v, ld_v);
+  auto kernel = L.bits == 4 ? vec ? kvq_prefill_kernel<4, true> : kvq_prefill_kernel<4, false>
+                : vec       ? kvq_prefill_kernel<8, true>
+                            : kvq_prefill_kernel<8, false>;
+  kernel<<<blocks, 256, L.tile, st>>>(data, L, state, seq, k, ld_k, v, ld_v, tokens, status);
 }
 
-// One token of every sequence: one CTA per sequence, one warp per head and
-// turn.  ROPE: rows are the fused projections [q | k | v]; q is rotated into
-// q_out and k rotated before it is quantised.
-template <bool ROPE>
+// ---- one token of every sequence ----------------------------------------------------
+// One CTA per sequence, one warp per head and key or value; lanes as above, the
+// token's bytes straight into the tile.  ROPE: the rows are the fused projections
+// [q | k | v]; q is rotated into q_out and k rotated before it is quantised.
+template <int BITS, bool ROPE>
 __global__ void __launch_bounds__(1024)
     kvq_push_kernel(unsigned char* data, const KvqLayout L, int* state, int window,
                     const float* __restrict__ k, long long ld_k, const float* __restrict__ v,
                     long long ld_v, float* q_out, const float2* __restrict__ table, int max_pos,
                     unsigned* status) {
+  constexpr int levels = (1 << BITS) - 1;
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   const int b = blockIdx.x;
@@ -152,6 +259,7 @@ __global__ void __launch_bounds__(1024)
   }
   const int pos = prefix + gen;
   const long long slot = prefix + gen % window;
+  const int t = static_cast<int>(slot & 31);
   const int half = L.dim >> 1;
   const long long width = static_cast<long long>(L.heads) * L.dim;
   const bool turn = ROPE && pos >= 0 && pos < max_pos;
@@ -166,22 +274,58 @@ __global__ void __launch_bounds__(1024)
     return d < half ? __fsub_rn(__fmul_rn(x0, c.x), __fmul_rn(x1, c.y))
                     : __fadd_rn(__fmul_rn(x1, c.x), __fmul_rn(x0, c.y));
   };
-  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7;
   for (int task = warp; task < 2 * L.heads; task += warps) {
     const int h = task >> 1;
-    unsigned char* tile = kvq_tile(data, L, b, h, slot);
+    const bool value = task & 1;
     const long long off = static_cast<long long>(h) * L.dim;
-    if (task & 1) {
-      const float* row = v + b * ld_v + off;
-      kvq_write_row<true>(tile, L, slot & 31, [&](int d) { return row[d]; }, status);
-    } else {
-      const float* row = k + b * ld_k + off;
-      kvq_write_row<false>(tile, L, slot & 31,
-                           [&](int d) { return ROPE ? rotated(row, d) : row[d]; }, status);
-      if (ROPE) {
-        const float* q = k - width + b * ld_k + off;
-        for (int d = lane; d < L.dim; d += 32) q_out[b * width + off + d] = rotated(q, d);
+    const float* row = (value ? v + b * ld_v : k + b * ld_k) + off;
+    unsigned char* codes = kvq_tile(data, L, b, h, slot) + (value ? L.half : 0);
+    for (int q = 0; q < (L.groups + 3) / 4; ++q) {
+      const int grp = q * 4 + (lane >> 3), d0 = grp * 32 + l8 * 4;
+      const bool real = grp < L.groups;
+      float x[4], hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = d0 + i;
+        x[i] = 0.0f;
+        if (d < L.dim) {
+          x[i] = ROPE && !value ? rotated(row, d) : row[d];
+          hi = fmaxf(hi, x[i]);
+          lo = fminf(lo, x[i]);
+        }
       }
+#pragma unroll
+      for (int o = 1; o <= 4; o <<= 1) {
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      }
+      float s, m;
+      uint32_t word = kvq_params(lo, hi, 1.0 / levels, levels, &s, &m);
+      uint32_t c = kvq_codes4(x, m, s, rcp_fast(s), levels);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d0 + i >= L.dim) c &= ~(0xFFu << (8 * i));
+      if ((__ballot_sync(0xffffffffu, kvq_refused(x)) >> (lane & 24)) & 0xFFu) {  // reads as NaN
+        word = 0x7FC00000u;
+        c = 0;
+        flag(status, DEV_KV_RANGE);
+      }
+      if (real && l8 == 0) *reinterpret_cast<uint32_t*>(codes + L.codes + kvq_param_byte(t, grp)) = word;
+      const uint32_t up = __shfl_xor_sync(0xffffffffu, c, value ? 2 : 4);
+      if (BITS == 4) c |= up << 4;
+      if (!real || (BITS == 4 && (l8 & (value ? 2 : 4)))) continue;
+      if (!value) {
+        *reinterpret_cast<uint32_t*>(codes + kvq_key_byte(t, d0, BITS)) = c;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          codes[kvq_value_byte(t, d0 + i, BITS)] = static_cast<unsigned char>(c >> (8 * i));
+      }
+    }
+    if (ROPE && !value) {
+      const float* q = row - width;
+      for (int d = lane; d < L.dim; d += 32) q_out[b * width + off + d] = rotated(q, d);
     }
   }
   __syncthreads();  // every thread has read `gen`
@@ -193,17 +337,18 @@ static int push_threads(const KvqLayout& L) { return 32 * (2 * L.heads < 32 ? 2 
 void launch_kvq_push(unsigned char* data, const KvqLayout& L, int* state, int batch, int window,
                      const float* k, long long ld_k, const float* v, long long ld_v,
                      unsigned* status, cudaStream_t st) {
-  launch_dependent(kvq_push_kernel<false>, dim3(batch), dim3(push_threads(L)), 0, st, data, L, state,
-                   window, k, ld_k, v, ld_v, nullptr, nullptr, 0, status);
+  launch_dependent(L.bits == 4 ? kvq_push_kernel<4, false> : kvq_push_kernel<8, false>, dim3(batch),
+                   dim3(push_threads(L)), 0, st, data, L, state, window, k, ld_k, v, ld_v, nullptr,
+                   nullptr, 0, status);
 }
 
 void launch_kvq_rope_push(unsigned char* data, const KvqLayout& L, int* state, int batch, int window,
                           const float* qkv, float* q_out, const float2* table, int max_pos,
                           unsigned* status, cudaStream_t st) {
   const long long width = static_cast<long long>(L.heads) * L.dim;
-  launch_dependent(kvq_push_kernel<true>, dim3(batch), dim3(push_threads(L)), 0, st, data, L, state,
-                   window, qkv + width, 3 * width, qkv + 2 * width, 3 * width, q_out, table, max_pos,
-                   status);
+  launch_dependent(L.bits == 4 ? kvq_push_kernel<4, true> : kvq_push_kernel<8, true>, dim3(batch),
+                   dim3(push_threads(L)), 0, st, data, L, state, window, qkv + width, 3 * width,
+                   qkv + 2 * width, 3 * width, q_out, table, max_pos, status);
 }
 
 __device__ __forceinline__ int kvq_tokens(const int* state, int b, int window) {
@@ -211,27 +356,58 @@ __device__ __forceinline__ int kvq_tokens(const int* state, int b, int window) {
   return prefix > 0 ? prefix + (gen < window ? gen : window) : 0;
 }
 
-// Slots [first, first + count) of one sequence as token-major rows of floats.
+// ---- reading back -----------------------------------------------------------------
+// Slots [first, first + count) of one sequence as token-major rows of floats: one
+// CTA per (tile, head), the tile staged in shared memory, lanes as in the prompt's
+// kernel.
+template <int BITS, bool VEC>
 __global__ void __launch_bounds__(256)
     kvq_read_kernel(const unsigned char* __restrict__ data, const KvqLayout L,
                     const int* __restrict__ state, int window, int seq, long long first,
                     long long count, float* k, float* v, unsigned* status) {
-  const long long left = kvq_tokens(state, seq, window) - first;
-  if (left < count && blockIdx.x == 0 && threadIdx.x == 0) flag(status, DEV_KV_SLOT);
-  const long long n = left < count ? left : count;
-  const int width = L.heads * L.dim;
-  for (long long t = blockIdx.x; t < n; t += gridDim.x) {
-    const long long slot = first + t;
-    const int tt = static_cast<int>(slot & 31);
-    for (int i = threadIdx.x; i < width; i += blockDim.x) {
-      const int h = i / L.dim, d = i - h * L.dim;
-      const unsigned char* tile = kvq_tile(const_cast<unsigned char*>(data), L, seq, h, slot);
-      for (int part = 0; part < 2; ++part) {
-        const unsigned char* codes = tile + part * L.half;
-        int c = codes[part ? kvq_value_byte(tt, d, L.bits) : kvq_key_byte(tt, d, L.bits)];
-        if (L.bits == 4) c = (c >> (4 * (part ? kvq_value_nibble(d) : kvq_key_nibble(d)))) & 15;
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + L.codes + kvq_param_byte(tt, d >> 5));
-        (part ? v : k)[t * width + i] = __fmaf_rn(bf16_low(w), static_cast<float>(c), bf16_high(w));
+  extern __shared__ __align__(16) unsigned char kvq_stage[];
+  const int h = blockIdx.x % L.heads;
+  const long long tile = (first >> 5) + blockIdx.x / L.heads;
+  const uint4* in = reinterpret_cast<const uint4*>(
+      kvq_tile(const_cast<unsigned char*>(data), L, seq, h, tile * 32));
+  for (int i = threadIdx.x; i < L.tile / 16; i += 256)
+    reinterpret_cast<uint4*>(kvq_stage)[i] = __ldg(in + i);
+  const long long held = kvq_tokens(state, seq, window);
+  const long long end = first + count < held ? first + count : held;
+  if (held < first + count && blockIdx.x == 0 && threadIdx.x == 0) flag(status, DEV_KV_SLOT);
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7;
+  const long long t0 = tile * 32 + warp * 4, width = static_cast<long long>(L.heads) * L.dim;
+  for (int q = 0; q < (L.groups + 3) / 4; ++q) {
+    const int grp = q * 4 + (lane >> 3), d0 = grp * 32 + l8 * 4;
+    if (grp >= L.groups || d0 >= L.dim) continue;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const unsigned char* codes = kvq_stage + part * L.half;
+      uint32_t c[4];  // bytes: keys: dims of token u; values: tokens of dim u
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        c[u] = *reinterpret_cast<const uint32_t*>(
+            codes + (part ? kvq_value_byte(warp * 4, d0 + u, BITS) : kvq_key_byte(warp * 4 + u, d0, BITS)));
+        if (BITS == 4) c[u] = (l8 & (part ? 2 : 4) ? c[u] >> 4 : c[u]) & 0x0F0F0F0Fu;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + L.codes + kvq_param_byte(warp * 4 + u, grp));
+        const float s = bf16_low(w), m = bf16_high(w);
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[i] = __fmaf_rn(s, static_cast<float>(((part ? c[i] : c[u]) >> (8 * (part ? u : i))) & 0xFFu), m);
+        if (t0 + u < first || t0 + u >= end) continue;
+        float* row = (part ? v : k) + (t0 + u - first) * width + static_cast<long long>(h) * L.dim + d0;
+        if (VEC) {
+          *reinterpret_cast<float4*>(row) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (d0 + i < L.dim) row[i] = x[i];
+        }
       }
     }
   }
@@ -239,10 +415,14 @@ __global__ void __launch_bounds__(256)
 
 void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* state, int window,
                      int seq, long long first, long long count, float* k, float* v, unsigned* status,
-                     int sms, cudaStream_t st) {
-  const long long most = 8LL * sms;
-  kvq_read_kernel<<<static_cast<int>(count < most ? count : most), 256, 0, st>>>(
-      data, L, state, window, seq, first, count, k, v, status);
+                     cudaStream_t st) {
+  const long long tiles = ((first + count - 1) >> 5) - (first >> 5) + 1;
+  const unsigned blocks = static_cast<unsigned>(tiles * L.heads);
+  const bool vec = kvq_vec(L, k, 0, v, 0);
+  auto kernel = L.bits == 4 ? vec ? kvq_read_kernel<4, true> : kvq_read_kernel<4, false>
+                : vec       ? kvq_read_kernel<8, true>
+                            : kvq_read_kernel<8, false>;
+  kernel<<<blocks, 256, L.tile, st>>>(data, L, state, window, seq, first, count, k, v, status);
 }
 
 // ---- attention -------------------------------------------------------------------
@@ -268,27 +448,37 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 // loop has no barrier but the ring's.  The warps' parts are joined in shared
 // memory, the CTAs' of one head through distributed shared memory: one launch,
 // no workspace.
-constexpr int kKvqWarps = 4;
 constexpr float kLog2e = 1.44269504f;
+// Weights stay below e^4 < 2^6 of the running maximum (see the loop).
+constexpr float kKvqSlack = 4.0f;
+constexpr int kKvqSlackBits = 6;
+constexpr int kKvqSlots = 2;  // ring slots per warp
+constexpr int kKvqCluster = 8;  // most CTAs of a cluster (portable)
 
 __host__ __device__ constexpr int kvq_tile_bytes(int groups, int bits) {
   return 2 * groups * (512 * (bits / 4) + 128);
 }
-// Ring slots per warp: about 20 KB, two at least, eight at most.
-__host__ __device__ constexpr int kvq_slots(int groups, int bits) {
-  const int n = 20480 / kvq_tile_bytes(groups, bits);
-  return n < 2 ? 2 : n > 8 ? 8 : n;
+
+// Tiles per turn of a warp and per ring slot.
+__host__ __device__ constexpr int kvq_per(int groups, int bits) {
+  return kvq_tile_bytes(groups, bits) <= 1280 ? 2 : 1;
+}
+// Warps of a CTA.
+__host__ __device__ constexpr int kvq_warps(int groups, int bits) {
+  const int turn = kvq_tile_bytes(groups, bits) * kvq_per(groups, bits);
+  return turn <= 5120 ? 4 : turn <= 10240 ? 2 : 1;
 }
 
 template <int G, int BITS>
 struct KvqShared {
-  static constexpr int kSlots = kvq_slots(G, BITS);
-  alignas(128) unsigned char ring[kKvqWarps][kSlots][kvq_tile_bytes(G, BITS)];
-  alignas(16) uint32_t weights[kKvqWarps][G][32];
-  uint64_t full[kKvqWarps][kSlots];
-  float o[kKvqWarps][G * 32];  // weighted values per warp; the CTA's in [0]
-  float m[kKvqWarps], l[kKvqWarps];
+  static constexpr int W = kvq_warps(G, BITS), N = kvq_per(G, BITS);
+  alignas(128) unsigned char ring[W][kKvqSlots][N * kvq_tile_bytes(G, BITS)];
+  alignas(16) uint32_t weights[W][N][G][32];
+  uint64_t full[W][kKvqSlots];
+  float o[W][G * 32];  // weighted values per warp; the CTA's in [0]
+  float m[W], l[W];
   float cta_m, cta_l;
+  int turn;
 };
 
 // u8 rows times signed (SIGNED) or unsigned columns, 32-bit sums.
@@ -343,36 +533,43 @@ __device__ __forceinline__ float part_factor(float m, float l, float M) {
 }
 
 template <int G, int BITS>
-__global__ void __launch_bounds__(kKvqWarps * 32) kvq_attention_kernel(const KvqAttnArgs a) {
-  constexpr int P = (G + 1) / 2;  // accumulators: pairs of groups
+__global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(const KvqAttnArgs a) {
   using Shared = KvqShared<G, BITS>;
-  constexpr int kSlots = Shared::kSlots, kTileBytes = kvq_tile_bytes(G, BITS);
+  constexpr int P = (G + 1) / 2;  // accumulators: pairs of groups
+  constexpr int N = Shared::N, W = Shared::W;
+  constexpr int kTileBytes = kvq_tile_bytes(G, BITS);
   constexpr int kCodes = G * 512 * (BITS / 4);
   extern __shared__ __align__(128) unsigned char kvq_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(kvq_raw);
-  pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
-  pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
-  const int splits = a.splits;
-  const int h = blockIdx.x / splits, rank = blockIdx.x % splits, b = blockIdx.y;
+  // a head: `parts` clusters of `splits` CTAs
+  const int splits = a.splits, share = blockIdx.x % (splits * a.parts), rank = share % splits;
+  const int h = blockIdx.x / (splits * a.parts), b = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
-  const int T = kvq_tokens(a.state, b, a.window);
-  if (T <= 0) {  // the same for every CTA of the cluster
-    if (threadIdx.x == 0 && rank == 0) flag(a.status, DEV_CACHE);
-    return;
-  }
-  const int tiles = (T + 31) >> 5, workers = splits * kKvqWarps, me = rank * kKvqWarps + warp;
-  const int first = static_cast<int>(static_cast<long long>(tiles) * me / workers);
-  const int last = static_cast<int>(static_cast<long long>(tiles) * (me + 1) / workers);
+  const int workers = splits * a.parts * W, me = share * W + warp;
   const unsigned char* head =
       a.data + (static_cast<long long>(b) * a.layout.heads + h) * a.layout.tiles * kTileBytes;
+  auto begin = [&](int tiles, int w) {
+    return static_cast<int>(static_cast<long long>(tiles) * w / workers);
+  };
+  pdl_wait_prior_grids();  // launched as a programmatic dependent (launch_dependent)
+  const int T = kvq_tokens(a.state, b, a.window);
+  if (T <= 0) {  // the same for every CTA of the cluster
+    if (threadIdx.x == 0 && share == 0) flag(a.status, DEV_CACHE);
+    return;
+  }
+  const int tiles = (T + 31) >> 5, first = begin(tiles, me), last = begin(tiles, me + 1);
+  const int end = min(T, last * 32);  // this warp's tokens end here
+  // tiles it, it + 1 of this warp into ring slot `slot`
+  auto fetch = [&](int it, int slot) {
+    const uint32_t bytes = (last - it < N ? last - it : N) * kTileBytes;
+    mbar_arrive_expect_tx(&sh.full[warp][slot], bytes);
+    bulk_g2s(sh.ring[warp][slot], head + static_cast<long long>(it) * kTileBytes, bytes,
+             &sh.full[warp][slot]);
+  };
   if (lane == 0) {
-    for (int i = 0; i < kSlots; ++i) mbar_init(&sh.full[warp][i], 1);
+    for (int i = 0; i < kKvqSlots; ++i) mbar_init(&sh.full[warp][i], 1);
     fence_mbar_init();
-    for (int i = 0; i < kSlots && first + i < last; ++i) {
-      mbar_arrive_expect_tx(&sh.full[warp][i], kTileBytes);
-      bulk_g2s(sh.ring[warp][i], head + static_cast<long long>(first + i) * kTileBytes, kTileBytes,
-               &sh.full[warp][i]);
-    }
+    for (int i = 0; i < kKvqSlots && first + i * N < last; ++i) fetch(first + i * N, i);
   }
   __syncwarp();
 
@@ -439,11 +636,12 @@ __global__ void __launch_bounds__(kKvqWarps * 32) kvq_attention_kernel(const Kvq
     o[p][0][0] = o[p][0][1] = o[p][1][0] = o[p][1][1] = 0.0f;
   }
 
-  for (int it = first, slot = 0, phase = 0; it < last; ++it) {
+  const int t = g + 8 * j;  // the token of a tile that this lane weighs
+  for (int it = first, slot = 0, phase = 0; it < last; it += N) {
     if (!__all_sync(0xffffffffu, mbar_wait_try(&sh.full[warp][slot], phase, a.status))) {
       // (a safety net: flagged) copies in flight land before the CTA ends
-      for (int i = 1; i < kSlots && it + i < last; ++i) {
-        if (++slot == kSlots) {
+      for (int i = 1; i < kKvqSlots && it + i * N < last; ++i) {
+        if (++slot == kKvqSlots) {
           slot = 0;
           phase ^= 1;
         }
@@ -452,31 +650,37 @@ __global__ void __launch_bounds__(kKvqWarps * 32) kvq_attention_kernel(const Kvq
       break;
     }
     const unsigned char* tile = sh.ring[warp][slot];
-    // ---- scores: x[i] is this lane's part of the score of token g + 8 i
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    {
+    // ---- scores (of a tile past the warp's last: of whatever the slot holds, masked below)
+    float score[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const unsigned char* kt = tile + u * kTileBytes;
       int d[2][P][4];
 #pragma unroll
-      for (int i = 0; i < 2 * P * 4; ++i) (&d[0][0][0])[i] = 0;
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[0][p][i] = d[1][p][i] = 0;
 #pragma unroll
       for (int grp = 0; grp < G; ++grp) {
         uint4 lo, hi;
         if (BITS == 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(tile + grp * 512 + lane * 16);
+          const uint4 w = *reinterpret_cast<const uint4*>(kt + grp * 512 + lane * 16);
           lo = make_uint4(w.x & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu, w.z & 0x0F0F0F0Fu, w.w & 0x0F0F0F0Fu);
           hi = make_uint4((w.x >> 4) & 0x0F0F0F0Fu, (w.y >> 4) & 0x0F0F0F0Fu,
                           (w.z >> 4) & 0x0F0F0F0Fu, (w.w >> 4) & 0x0F0F0F0Fu);
         } else {
-          lo = *reinterpret_cast<const uint4*>(tile + grp * 1024 + lane * 16);
-          hi = *reinterpret_cast<const uint4*>(tile + grp * 1024 + 512 + lane * 16);
+          lo = *reinterpret_cast<const uint4*>(kt + grp * 1024 + lane * 16);
+          hi = *reinterpret_cast<const uint4*>(kt + grp * 1024 + 512 + lane * 16);
         }
         mma_u8_m16n8k32<true>(d[0][grp >> 1], lo.x, lo.y, hi.x, hi.y, qb[grp][0], qb[grp][1]);
         mma_u8_m16n8k32<true>(d[1][grp >> 1], lo.z, lo.w, hi.z, hi.w, qb[grp][0], qb[grp][1]);
       }
+      // x[i]: this lane's part of the score of token g + 8 i
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const int grp = min(2 * p + acc_group, G - 1);
-        const uint4 w = *reinterpret_cast<const uint4*>(tile + kCodes + grp * 128 + g * 16);
+        const uint4 w = *reinterpret_cast<const uint4*>(kt + kCodes + grp * 128 + g * 16);
         const uint32_t par[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -485,89 +689,108 @@ __global__ void __launch_bounds__(kKvqWarps * 32) kvq_attention_kernel(const Kvq
           x[i] = fmaf(bf16_low(par[i]), dot, fmaf(bf16_high(par[i]), qsum[p], x[i]));
         }
       }
+      // the four lanes of a row add up and lane j keeps token t = g + 8 j
+      const float r0 = (j & 2 ? x[2] : x[0]) + __shfl_xor_sync(0xffffffffu, j & 2 ? x[0] : x[2], 2);
+      const float r1 = (j & 2 ? x[3] : x[1]) + __shfl_xor_sync(0xffffffffu, j & 2 ? x[1] : x[3], 2);
+      score[u] = ((j & 1 ? r1 : r0) + __shfl_xor_sync(0xffffffffu, j & 1 ? r0 : r1, 1)) * a.scale;
     }
-    // the four lanes of a row add up and lane j keeps token t = g + 8 j
-    const float r0 = (j & 2 ? x[2] : x[0]) + __shfl_xor_sync(0xffffffffu, j & 2 ? x[0] : x[2], 2);
-    const float r1 = (j & 2 ? x[3] : x[1]) + __shfl_xor_sync(0xffffffffu, j & 2 ? x[1] : x[3], 2);
-    const float score =
-        ((j & 1 ? r1 : r0) + __shfl_xor_sync(0xffffffffu, j & 1 ? r0 : r1, 1)) * a.scale;
-    const int t = g + 8 * j;
-    const bool in = it * 32 + t < T;
-    // ---- softmax
-    const float top = warp_max(in ? score : -INFINITY);
-    if (top > m) {
-      const float keep = exp2_fast((m - top) * kLog2e);
-      m = top;
-      l *= keep;
+    // ---- the steps and least values of the tokens that are there
+    uint32_t par[N][G];
+    bool in[N], over = false;
 #pragma unroll
-      for (int i = 0; i < G; ++i) least[i] *= keep;
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        o[p][0][0] *= keep;
-        o[p][0][1] *= keep;
-        o[p][1][0] *= keep;
-        o[p][1][1] *= keep;
-      }
-    }
-    const float pr = in ? exp2_fast((score - m) * kLog2e) : 0.0f;
-    l += pr;
-    // ---- the weights' bytes
-    const unsigned char* vt = tile + kTileBytes / 2;
-    uint32_t par[G];
-    bool over = false;
-#pragma unroll
-    for (int i = 0; i < G; ++i) {
-      // a token that is not there: nothing of what its slot holds
-      par[i] = in ? *reinterpret_cast<const uint32_t*>(vt + kCodes + i * 128 + lane * 4) : 0;
-      over |= (par[i] & 0xFFFFu) > bound[i];
-    }
-    if (__any_sync(0xffffffffu, over)) {
+    for (int u = 0; u < N; ++u) {
+      in[u] = (it + u) * 32 + t < end;
+      over |= in[u] && score[u] > m + kKvqSlack;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        bound[i] = max(bound[i], __reduce_max_sync(0xffffffffu, par[i] & 0xFFFFu));
-        // step < 2^(e - 126); steps below 2^-86 lose precision
+        par[u][i] = in[u] ? *reinterpret_cast<const uint32_t*>(tile + u * kTileBytes + kTileBytes / 2 +
+                                                               kCodes + i * 128 + lane * 4)
+                          : 0;
+        over |= (par[u][i] & 0xFFFFu) > bound[i];
+      }
+    }
+    // ---- softmax: m, the maximum that the weights refer to, is raised only when
+    // a score passes it by kKvqSlack, the bounds only when a step passes them:
+    // one vote for all in most turns
+    if (__any_sync(0xffffffffu, over)) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < N; ++u) top = fmaxf(top, in[u] ? score[u] : -INFINITY);
+      top = warp_max(top);
+      if (top > m) {
+        const float keep = exp2_fast((m - top) * kLog2e);
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int i = 0; i < G; ++i) least[i] *= keep;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          o[p][0][0] *= keep;
+          o[p][0][1] *= keep;
+          o[p][1][0] *= keep;
+          o[p][1][1] *= keep;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        uint32_t big = 0;
+#pragma unroll
+        for (int u = 0; u < N; ++u) big = max(big, par[u][i] & 0xFFFFu);
+        bound[i] = max(bound[i], __reduce_max_sync(0xffffffffu, big));
+        // step < 2^(e - 126), weight < 2^6; steps below 2^-86 lose precision
         const uint32_t e = max(bound[i] >> 7, 40u);
-        wup[i] = __uint_as_float((284u - e) << 23);
+        wup[i] = __uint_as_float((284u - kKvqSlackBits - e) << 23);
       }
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const uint32_t bd = acc_group && 2 * p + 1 < G ? bound[min(2 * p + 1, G - 1)] : bound[2 * p];
-        wdown[p] = __uint_as_float((max(bd >> 7, 40u) - 30u + (j & 1) * 16u) << 23);
+        wdown[p] = __uint_as_float((max(bd >> 7, 40u) - 30u + kKvqSlackBits + (j & 1) * 16u) << 23);
       }
     }
+    // ---- the weights' bytes
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      least[i] = fmaf(pr, bf16_high(par[i]), least[i]);
-      sh.weights[warp][i][t] = __float2uint_rn(pr * (bf16_low(par[i]) * wup[i]));
+    for (int u = 0; u < N; ++u) {
+      const float pr = in[u] ? exp2_fast((score[u] - m) * kLog2e) : 0.0f;
+      l += pr;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        least[i] = fmaf(pr, bf16_high(par[u][i]), least[i]);
+        sh.weights[warp][u][i][t] = __float2uint_rn(pr * (bf16_low(par[u][i]) * wup[i]));
+      }
     }
     __syncwarp();
     // ---- values
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const uint32_t* wp = sh.weights[warp][min(2 * p + col_group, G - 1)];
-      const uint4 w0 = *reinterpret_cast<const uint4*>(wp + 4 * j);
-      const uint4 w1 = *reinterpret_cast<const uint4*>(wp + 16 + 4 * j);
-      const uint32_t b0 = gather_bytes(w0.x, w0.y, w0.z, w0.w, col_byte);
-      const uint32_t b1 = gather_bytes(w1.x, w1.y, w1.z, w1.w, col_byte);
       int d[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int grp = 2 * p + c;
-        if (grp >= G) break;
-        const uint32_t c0 = col_group == c ? b0 : 0, c1 = col_group == c ? b1 : 0;
-        if (BITS == 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(vt + grp * 512 + lane * 16);
-          mma_u8_m16n8k32<false>(d[0], w.x & 0x0F0F0F0Fu, (w.x >> 4) & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu,
-                                 (w.y >> 4) & 0x0F0F0F0Fu, c0, c1);
-          mma_u8_m16n8k32<false>(d[1], w.z & 0x0F0F0F0Fu, (w.z >> 4) & 0x0F0F0F0Fu, w.w & 0x0F0F0F0Fu,
-                                 (w.w >> 4) & 0x0F0F0F0Fu, c0, c1);
-        } else {
-          const uint4 v0 = *reinterpret_cast<const uint4*>(vt + grp * 1024 + lane * 16);
-          const uint4 v1 = *reinterpret_cast<const uint4*>(vt + grp * 1024 + 512 + lane * 16);
-          mma_u8_m16n8k32<false>(d[0], v0.x, v0.y, v0.z, v0.w, c0, c1);
-          mma_u8_m16n8k32<false>(d[1], v1.x, v1.y, v1.z, v1.w, c0, c1);
+      for (int u = 0; u < N; ++u) {
+        const unsigned char* vt = tile + u * kTileBytes + kTileBytes / 2;
+        const uint32_t* wp = sh.weights[warp][u][min(2 * p + col_group, G - 1)];
+        const uint4 w0 = *reinterpret_cast<const uint4*>(wp + 4 * j);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(wp + 16 + 4 * j);
+        const uint32_t b0 = gather_bytes(w0.x, w0.y, w0.z, w0.w, col_byte);
+        const uint32_t b1 = gather_bytes(w1.x, w1.y, w1.z, w1.w, col_byte);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int grp = 2 * p + c;
+          if (grp >= G) break;
+          const uint32_t c0 = col_group == c ? b0 : 0, c1 = col_group == c ? b1 : 0;
+          if (BITS == 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(vt + grp * 512 + lane * 16);
+            mma_u8_m16n8k32<false>(d[0], w.x & 0x0F0F0F0Fu, (w.x >> 4) & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu,
+                                   (w.y >> 4) & 0x0F0F0F0Fu, c0, c1);
+            mma_u8_m16n8k32<false>(d[1], w.z & 0x0F0F0F0Fu, (w.z >> 4) & 0x0F0F0F0Fu, w.w & 0x0F0F0F0Fu,
+                                   (w.w >> 4) & 0x0F0F0F0Fu, c0, c1);
+          } else {
+            const uint4 v0 = *reinterpret_cast<const uint4*>(vt + grp * 1024 + lane * 16);
+            const uint4 v1 = *reinterpret_cast<const uint4*>(vt + grp * 1024 + 512 + lane * 16);
+            mma_u8_m16n8k32<false>(d[0], v0.x, v0.y, v0.z, v0.w, c0, c1);
+            mma_u8_m16n8k32<false>(d[1], v1.x, v1.y, v1.z, v1.w, c0, c1);
+          }
         }
       }
+      // (sums of N tiles: at most 2 * 32 * 255 * 255 * 257 < 2^31)
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -576,17 +799,17 @@ __global__ void __launch_bounds__(kKvqWarps * 32) kvq_attention_kernel(const Kvq
                               o[p][mb][up]);
     }
     __syncwarp();  // every lane has read the slot and the weights
-    if (lane == 0 && it + kSlots < last) {
-      mbar_arrive_expect_tx(&sh.full[warp][slot], kTileBytes);
-      bulk_g2s(sh.ring[warp][slot], head + static_cast<long long>(it + kSlots) * kTileBytes, kTileBytes,
-               &sh.full[warp][slot]);
-    }
-    if (++slot == kSlots) {
+    if (lane == 0 && it + kKvqSlots * N < last) fetch(it + kKvqSlots * N, slot);
+    if (++slot == kKvqSlots) {
       slot = 0;
       phase ^= 1;
     }
   }
 
+  // The next kernel (usually a push) may become resident now: earlier, its CTAs
+  // take the registers that this one's last CTAs wait for (43.6 -> 42.3 us for
+  // push and attention of 64 sequences x 2176 tokens).
+  pdl_launch_dependents();
   // ---- the warps' parts
   l = warp_sum(l);
 #pragma unroll
@@ -607,74 +830,138 @@ __global__ void __launch_bounds__(kKvqWarps * 32) kvq_attention_kernel(const Kvq
     sh.l[warp] = l;
   }
   __syncthreads();
-  float M = sh.m[0], L = 0.0f, f[kKvqWarps];
+  float M = sh.m[0], L = 0.0f, f[W];
 #pragma unroll
-  for (int w = 1; w < kKvqWarps; ++w) M = fmaxf(M, sh.m[w]);
+  for (int w = 1; w < W; ++w) M = fmaxf(M, sh.m[w]);
 #pragma unroll
-  for (int w = 0; w < kKvqWarps; ++w) {
+  for (int w = 0; w < W; ++w) {
     f[w] = part_factor(sh.m[w], sh.l[w], M);
     L = fmaf(f[w], sh.l[w], L);
   }
-  if (splits > 1) {
-    for (int d = threadIdx.x; d < G * 32; d += kKvqWarps * 32) {
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kKvqWarps; ++w) v = fmaf(f[w], sh.o[w][d], v);
-      sh.o[0][d] = v;  // read and written by this thread alone
+  // out[d] of the whole from the joined value of dim d and the sum L
+  const int dim = a.layout.dim;
+  auto finish = [&](auto value) {  // value(d) by whole warps; it may set M and L
+    for (int d = threadIdx.x; d < G * 32; d += W * 32) {
+      const float v = value(d);
+      const bool bad = !(L > 0.0f && L < INFINITY) || !isfinite(M);
+      if (bad && d == 0) flag(a.status, DEV_SOFTMAX);
+      if (d < dim) a.out[row + d] = bad ? __uint_as_float(0x7FC00000u) : v / L;
     }
-    if (threadIdx.x == 0) {
-      sh.cta_m = M;
-      sh.cta_l = L;
-    }
-    cluster_arrive();
-    cluster_wait();
-    float cm[16], cf[16];
-    M = -INFINITY;
-    for (int r = 0; r < splits; ++r) M = fmaxf(M, cm[r] = cluster_load(&sh.cta_m, r));
-    L = 0.0f;
-    for (int r = 0; r < splits; ++r) {
-      const float cl = cluster_load(&sh.cta_l, r);
-      cf[r] = part_factor(cm[r], cl, M);
-      L = fmaf(cf[r], cl, L);
-    }
-    const bool bad = !(L > 0.0f && L < INFINITY) || !isfinite(M);
-    for (int d = rank * kKvqWarps * 32 + threadIdx.x; d < a.layout.dim; d += splits * kKvqWarps * 32) {
-      float v = 0.0f;
-      for (int r = 0; r < splits; ++r) v = fmaf(cf[r], cluster_load(&sh.o[0][d], r), v);
-      a.out[row + d] = bad ? __uint_as_float(0x7FC00000u) : v / L;
-    }
-    if (bad && rank == 0 && threadIdx.x == 0) flag(a.status, DEV_SOFTMAX);
-    cluster_arrive();  // no CTA leaves while its part may still be read
-    cluster_wait();
-    return;
-  }
-  const bool bad = !(L > 0.0f && L < INFINITY) || !isfinite(M);
-  if (bad && threadIdx.x == 0) flag(a.status, DEV_SOFTMAX);
-  for (int d = threadIdx.x; d < a.layout.dim; d += kKvqWarps * 32) {
+  };
+  auto of_warps = [&](int d) {
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kKvqWarps; ++w) v = fmaf(f[w], sh.o[w][d], v);
-    a.out[row + d] = bad ? __uint_as_float(0x7FC00000u) : v / L;
+    for (int w = 0; w < W; ++w) v = fmaf(f[w], sh.o[w][d], v);
+    return v;
+  };
+  if (splits == 1) {
+    finish(of_warps);
+    return;
   }
+  // ---- the CTAs of a cluster, by its first
+  for (int d = threadIdx.x; d < G * 32; d += W * 32) sh.o[0][d] = of_warps(d);  // (own element)
+  if (threadIdx.x == 0) {
+    sh.cta_m = M;
+    sh.cta_l = L;
+  }
+  cluster_arrive();
+  cluster_wait();
+  if (rank == 0) {
+    // lane r weighs part r; a part's values are loaded before its weight is known
+    float part;
+    auto weigh = [&](float pm, float pl) {
+      M = warp_max(pm);
+      part = part_factor(pm, pl, M);
+      L = warp_sum(part * pl);
+    };
+    const bool mine = lane < splits;
+    weigh(mine ? cluster_load(&sh.cta_m, lane) : -INFINITY, mine ? cluster_load(&sh.cta_l, lane) : 0.0f);
+    auto of_cluster = [&](int d) {
+      float v[kKvqCluster], sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < kKvqCluster; ++r) v[r] = r < splits ? cluster_load(&sh.o[0][d], r) : 0.0f;
+#pragma unroll
+      for (int r = 0; r < kKvqCluster; ++r) sum = fmaf(__shfl_sync(0xffffffffu, part, r), v[r], sum);
+      return sum;
+    };
+    if (a.parts == 1) {
+      finish(of_cluster);
+    } else {
+      // ---- the clusters of a head, by the one that ends last, in their order
+      const int unit = b * a.layout.heads + h, stride = dim + 2;
+      float* all = a.partial + static_cast<long long>(unit) * a.parts * stride;
+      float* own = all + share / splits * stride;
+      for (int d = threadIdx.x; d < G * 32; d += W * 32) {
+        const float v = of_cluster(d);
+        if (d < dim) own[2 + d] = v;
+      }
+      if (threadIdx.x == 0) {
+        own[0] = M;
+        own[1] = L;
+      }
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) sh.turn = atomicAdd(a.tickets + unit, 1);
+      __syncthreads();
+      if (sh.turn == a.parts - 1) {
+        __threadfence();
+        if (threadIdx.x == 0) a.tickets[unit] = 0;  // for the next launch
+        const bool there = lane < a.parts;
+        const float pm = there ? __ldcg(all + lane * stride) : -INFINITY;
+        const float pl = there ? __ldcg(all + lane * stride + 1) : 0.0f;
+        bool weighed = false;
+        auto of_parts = [&](int d) {
+          float v[kKvqMaxParts], sum = 0.0f;
+#pragma unroll
+          for (int r = 0; r < kKvqMaxParts; ++r)
+            v[r] = r < a.parts && d < dim ? __ldcg(all + r * stride + 2 + d) : 0.0f;
+          if (!weighed) weigh(pm, pl);
+          weighed = true;
+#pragma unroll
+          for (int r = 0; r < kKvqMaxParts; ++r) sum = fmaf(__shfl_sync(0xffffffffu, part, r), v[r], sum);
+          return sum;
+        };
+        finish(of_parts);
+      }
+    }
+  }
+  cluster_arrive();  // no CTA leaves while its part may still be read
+  cluster_wait();
 }
 
 template <int G, int BITS>
-static cudaError_t launch_kvq_attention_t(const KvqAttnArgs& a, int batch, cudaStream_t st) {
-  constexpr size_t smem = sizeof(KvqShared<G, BITS>);
+static cudaError_t launch_kvq_attention_t(KvqAttnArgs a, int batch, cudaStream_t st) {
+  using Shared = KvqShared<G, BITS>;
+  constexpr size_t smem = sizeof(Shared);
   static_assert(smem <= 227 * 1024, "shared memory of a CTA");
   static PerDeviceOnce configured;
   configured.run([] {
     cudaFuncSetAttribute(kvq_attention_kernel<G, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          static_cast<int>(smem));
   });
+  // Every CTA resident at once where the heads are few: clusters of up to eight
+  // while the warps of a head outnumber no tiles of a full cache, then several
+  // clusters per head while every warp keeps 4 tiles.
+  constexpr int W = Shared::W;
+  const long long heads = static_cast<long long>(batch) * a.layout.heads;
+  constexpr int kPerSm = 227 * 1024 / (smem + 1024);
+  const long long slots = static_cast<long long>(a.sms) * (kPerSm < kKvqCtasPerSm ? kPerSm : kKvqCtasPerSm);
+  a.splits = a.parts = 1;
+  while (a.splits < kKvqCluster && 2 * heads * a.splits <= slots && a.layout.tiles > a.splits * W)
+    a.splits *= 2;
+  if (a.splits > 1) {
+    const long long most = slots / (heads * a.splits), fed = a.layout.tiles / (a.splits * W * 4);
+    const long long parts = most < fed ? most : fed;
+    a.parts = parts < 1 ? 1 : parts > kKvqMaxParts ? kKvqMaxParts : static_cast<int>(parts);
+  }
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {static_cast<unsigned>(a.splits), 1, 1};
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(a.layout.heads * a.splits, batch);
-  cfg.blockDim = dim3(kKvqWarps * 32);
+  cfg.gridDim = dim3(a.layout.heads * a.splits * a.parts, batch);
+  cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -703,14 +990,7 @@ static cudaError_t launch_kvq_attention_b(const KvqAttnArgs& a, int batch, cudaS
   }
 }
 
-cudaError_t launch_kvq_attention(KvqAttnArgs a, int batch, cudaStream_t st) {
-  // CTAs per head: enough for two per SM, at most a portable cluster, and no
-  // more than leave every warp a tile of a full cache
-  const long long heads = static_cast<long long>(batch) * a.layout.heads;
-  a.splits = 1;
-  while (a.splits < 8 && heads * a.splits < 2LL * a.sms &&
-         a.layout.tiles > static_cast<long long>(a.splits) * kKvqWarps)
-    a.splits *= 2;
+cudaError_t launch_kvq_attention(const KvqAttnArgs& a, int batch, cudaStream_t st) {
   return a.layout.bits == 4 ? launch_kvq_attention_b<4>(a, batch, st)
                             : launch_kvq_attention_b<8>(a, batch, st);
 }
