@@ -396,9 +396,10 @@ struct LogprobArgs {
   long long* top_ids;        // [rows][top_k], or null when top_k is 0
   float* top_logprobs;       // the same
   unsigned* status;
+  int splits;                // CTAs per row: set by the launcher
 };
 constexpr int kLogprobMaxTop = 32;
-cudaError_t launch_token_logprobs(const LogprobArgs& a, int rows, int sms, cudaStream_t st);
+cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t st);
 
 // rope_table.cpp — host: the reference's cos/sin of every (position, pair).
 void build_rope_table(int dim, float theta, int max_pos, float* cos_sin /* [max_pos][dim/2][2] */);
