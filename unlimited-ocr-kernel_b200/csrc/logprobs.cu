@@ -9,26 +9,31 @@
 // nearly certain token and a nearly zero entropy exact to a float's relative
 // precision, and both terms of H are >= 0, so nothing cancels.
 //
-// One pass: every thread keeps the maximum of what it has seen, the sums that
-// refer to it, and rescales them once per 16 elements.  The alternatives are
-// those of a short list of candidates per CTA: an element enters it when its
-// key (logit, then lower index) reaches the k-th best one known.  A first bound
-// comes from the threads' maxima (k of them reach it, so k elements do); the
-// list is cut back to its k best, in order, whenever it grows, which raises the
-// bound.  A row is spread over a cluster of CTAs where the rows are few; the
-// CTAs' sums and lists are joined through distributed shared memory.
+// One pass: every warp keeps the maximum of what it has seen and sums that refer
+// to it; a new maximum, a rare thing, rescales them.  The alternatives come
+// from a short list of candidates per CTA: an element joins when its key (logit,
+// then lower index) reaches a bound that k keys are known to reach.  The first
+// bound comes from the first segment's threads' maxima, the next ones from
+// cutting the list back to its k best after segments 1, 4, 16, 64, ...; in
+// between no warp waits for another.  Where that list runs full (logits that
+// rise along the row, thousands of equal ones), or fewer than k logits are
+// finite, the alternatives are picked in a second pass that bounds every
+// segment exactly.  A row is spread over a cluster of CTAs where the rows are
+// few; the CTAs' sums and lists are joined through distributed shared memory.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
+#include "device_once.h"
 #include "kernels.h"
 
 namespace uocr {
 
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpVec = 4;                    // 16-byte loads per thread and segment
-constexpr int kLpPer = 4 * kLpVec;           // elements per thread and segment
-constexpr int kLpSegment = kLpThreads * kLpVec;  // 16-byte vectors
+constexpr int kLpVec = 4;                    // 16-byte vectors per lane and turn
+constexpr int kLpPer = 4 * kLpVec;           // elements per lane and turn
+constexpr int kLpTurn = 32 * kLpVec;         // vectors per warp and turn: one bulk copy
+constexpr int kLpStages = 3;                 // ring slots per warp
 constexpr int kLpCluster = 8;                // most CTAs per row (portable)
 // Candidates: at most kLpCut stay after a cut, kLogprobMaxTop threads' elements
 // join by the exact bound.
@@ -59,31 +64,48 @@ __device__ __forceinline__ float lp_exp2(float x) {  // 2 ulp
   return y;
 }
 
-struct alignas(16) LpShared {
-  LpKey list[2][kLpList];
-  LpKey best[kLpCluster * kLogprobMaxTop];  // the CTA's best; the row's parts in the first CTA
-  float m[kLpWarps], s[kLpWarps], w[kLpWarps], n[kLpWarps];
-  float part[4];                   // the CTA's {M, S, W, n}
-  uint32_t bound[kLpWarps];
-  int count[2];
+struct LpShared {
+  alignas(128) float4 ring[kLpWarps][kLpStages][kLpTurn];
+  alignas(16) LpKey list[kLpList];
+  alignas(16) LpKey keys[kLpThreads];        // the threads' best; the parts' lists of a row
+  LpKey best[kLogprobMaxTop];                // the k best of a cut, in order
   LpKey floor;
+  uint64_t full[kLpWarps][kLpStages];
+  float m[kLpWarps], s[kLpWarps], w[kLpWarps], n[kLpWarps];
+  float part[4];                             // the CTA's {M, S, W, n}
+  uint32_t bound[kLpWarps];
+  int count;                                 // candidates that have joined
+  int over;                                  // more than the list holds
 };
 
-// The k best of list[from][0, n), in order, into dst; the k-th best (0 while
-// there are fewer) is the new floor.  All threads; a barrier before and after.
-__device__ __forceinline__ void lp_cut(LpShared& sh, const LpKey* src, int n, int k, LpKey* dst) {
+// The k best of src[0, n), in order, into sh.best; the k-th best, where there
+// are k, is the new floor.  All threads; a barrier before and after.
+__device__ __forceinline__ void lp_rank(LpShared& sh, const LpKey* src, int n, int k) {
+#pragma unroll 1
   for (int i = threadIdx.x; i < n; i += kLpThreads) {
     const LpKey mine = src[i];
-    int rank = 0;
-    int c = 0;
-    for (; c + 2 <= n; c += 2) {
-      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(src + c);
-      rank += (o.x > mine) + (o.y > mine);
+    int rank = 0, c = 0;
+#pragma unroll 1
+    for (; c + 8 <= n; c += 8) {
+      ulonglong2 o[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o[u] = *reinterpret_cast<const ulonglong2*>(src + c + 2 * u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) rank += (o[u].x > mine) + (o[u].y > mine);
     }
-    if (c < n) rank += src[c] > mine;
-    if (rank < k) dst[rank] = mine;
+#pragma unroll 1
+    for (; c < n; ++c) rank += src[c] > mine;
+    if (rank < k) sh.best[rank] = mine;
     if (rank == k - 1) sh.floor = mine;
   }
+}
+
+// The list cut back to its k best (n > k of them).  All threads, between barriers.
+__device__ __noinline__ void lp_cut(LpShared& sh, int n, int k) {
+  lp_rank(sh, sh.list, n, k);
+  __syncthreads();
+  if (threadIdx.x < k) sh.list[threadIdx.x] = sh.best[threadIdx.x];
+  if (threadIdx.x == 0) sh.count = k;
 }
 
 __device__ __forceinline__ uint32_t lp_mapped(const void* p, uint32_t rank) {
@@ -102,7 +124,8 @@ __device__ __forceinline__ LpKey lp_remote(const LpKey* p, uint32_t rank) {
   return v;
 }
 
-// Sums {S, W, n} that refer to a maximum m, as they stand to M >= m.
+// Sums S = sum e^{x - m} over all elements but n that equal m, and W = sum
+// e^{x - m} (x - m), as they stand to a maximum M >= m.
 __device__ __forceinline__ void lp_refer(float m, float M, float& s, float& w, float& n) {
   if (m == M) return;
   const float d = fmaxf(m - M, -1000.0f), f = lp_exp2(d * kLpLog2e), all = s + n;
@@ -111,163 +134,283 @@ __device__ __forceinline__ void lp_refer(float m, float M, float& s, float& w, f
   n = 0.0f;
 }
 
+__device__ __forceinline__ float lp_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float lp_max_nan(float a, float b) {  // NaN where one is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// One CTA's elements [e0, e1) of a row: whole 16-byte vectors, and where the row
+// does not start or end with one, up to three elements at either end.
+struct LpRow {
+  const float* x;
+  int e0, e1;
+  int head, tail;  // elements ahead of the vectors and behind them
+  int vecs;        // vectors from element e0 + head
+
+  // Element i of the warp's turn `it` (after the vectors' turns: the ends), as an
+  // index of the row.
+  __device__ __forceinline__ int index(int it, int turns, int i) const {
+    const int lane = threadIdx.x & 31;
+    if (it >= turns) return lane < head ? e0 + lane : e1 - tail + lane - head;
+    return e0 + head + 4 * ((it * kLpWarps + (threadIdx.x >> 5)) * kLpTurn + (i >> 2) * 32 + lane) + (i & 3);
+  }
+};
+
+// The hits of a turn (bits: elements of this lane) join the list: one place per
+// warp, its lanes' elements next to each other.  Their logits are read again: a
+// rare call with as little code in the loop as can be.
+__device__ __noinline__ void lp_join(LpShared& sh, const LpRow& row, int it, int turns, uint32_t hits) {
+  const int lane = threadIdx.x & 31, mine = __popc(hits);
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int below = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += below;
+  }
+  int at = 0;
+  if (lane == 31) at = atomicAdd(&sh.count, upto);
+  at = __shfl_sync(0xffffffffu, at, 31) + upto - mine;
+#pragma unroll 1
+  for (; hits; hits &= hits - 1, ++at) {
+    const int e = row.index(it, turns, __ffs(hits) - 1);
+    if (at < kLpList) sh.list[at] = lp_key(__ldg(row.x + e), e);
+  }
+}
+
+// The r-th best of every warp's 32 orders, r = ceil(k / warps): k threads reach
+// the least of them, and so do k elements.  A barrier before and after.
+__device__ __noinline__ void lp_bound(LpShared& sh, uint32_t order, int k) {
+  uint32_t nth = 0;
+#pragma unroll 1
+  for (int r = 0; r < (k + kLpWarps - 1) / kLpWarps; ++r) {
+    nth = __reduce_max_sync(0xffffffffu, order);
+    const unsigned who = __ballot_sync(0xffffffffu, order == nth);
+    if ((threadIdx.x & 31) == __ffs(who) - 1) order = 0;
+  }
+  if ((threadIdx.x & 31) == 0) sh.bound[threadIdx.x >> 5] = nth;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t low = sh.bound[0];
+#pragma unroll
+    for (int i = 1; i < kLpWarps; ++i) low = min(low, sh.bound[i]);
+    sh.floor = static_cast<LpKey>(low) << 32;
+  }
+  __syncthreads();
+}
+
+// The candidates of the CTA's elements picked again, whatever the logits are:
+// every 4096 elements bounded by the k-th best of the threads' best keys, which
+// only k threads reach.  The list ends with all of the k best in it.
+__device__ __noinline__ void lp_pick_exactly(LpShared& sh, const LpRow& row, int k) {
+  const int tid = threadIdx.x;
+  if (tid == 0) sh.count = 0;
+#pragma unroll 1
+  for (int first = row.e0; first < row.e1; first += kLpThreads * kLpPer) {
+    LpKey best = 0;
+#pragma unroll 4
+    for (int i = 0; i < kLpPer; ++i) {
+      const int e = first + i * kLpThreads + tid;
+      const float v = e < row.e1 ? __ldg(row.x + e) : 0.0f;
+      const LpKey key = e < row.e1 && !isnan(v) ? lp_key(v, e) : 0;
+      best = key > best ? key : best;
+    }
+    __syncthreads();
+    sh.keys[tid] = best;
+    __syncthreads();
+    int above = 0;
+#pragma unroll 4
+    for (int c = 0; c < kLpThreads; c += 2) {
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(sh.keys + c);
+      above += (o.x > best) + (o.y > best);
+    }
+    if (above == k - 1 && best > sh.floor) sh.floor = best;  // (one thread, the only reader)
+    __syncthreads();
+    const LpKey floor = sh.floor;
+    if (best >= floor) {
+#pragma unroll 1
+      for (int i = 0; i < kLpPer; ++i) {
+        const int e = first + i * kLpThreads + tid;
+        if (e >= row.e1) break;
+        const float v = __ldg(row.x + e);
+        const LpKey key = isnan(v) ? 0 : lp_key(v, e);
+        if (key != 0 && key >= floor) sh.list[atomicAdd(&sh.count, 1)] = key;
+      }
+    }
+    __syncthreads();
+    const int held = sh.count;
+    __syncthreads();
+    if (held > kLpCut) lp_cut(sh, held, k);  // room for the next 4096's
+  }
+  __syncthreads();
+}
+
 template <bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LogprobArgs a) {
-  __shared__ LpShared sh;
+__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const LogprobArgs a) {
+  extern __shared__ __align__(128) unsigned char lp_raw[];
+  LpShared& sh = *reinterpret_cast<LpShared*>(lp_raw);
+  pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
+  pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   const int splits = a.splits, rank = blockIdx.x % splits, row = blockIdx.x / splits;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.top_k;
-  const float* x = a.logits + row * a.ld;
+  LpRow part;
+  part.x = a.logits + row * a.ld;
+  {
+    const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(part.x) >> 2) & 3);
+    const int head = skip ? min(4 - skip, a.vocab) : 0;
+    const int vecs = (a.vocab - head) >> 2;  // of the row
+    const int first = static_cast<int>(static_cast<long long>(vecs) * rank / splits);
+    const int last = static_cast<int>(static_cast<long long>(vecs) * (rank + 1) / splits);
+    part.vecs = last - first;
+    part.head = rank == 0 ? head : 0;
+    part.tail = rank == splits - 1 ? a.vocab - head - 4 * vecs : 0;
+    part.e0 = rank == 0 ? 0 : head + 4 * first;
+    part.e1 = rank == splits - 1 ? a.vocab : head + 4 * last;
+  }
+  // turns of every warp: a bulk copy of up to kLpTurn vectors each; one more for
+  // the elements at the ends
+  const int turns = (part.vecs + kLpWarps * kLpTurn - 1) / (kLpWarps * kLpTurn);
+  const int all_turns = turns + (part.head + part.tail > 0);
+  auto vectors = [&](int it) {  // of this warp's turn
+    return max(0, min(kLpTurn, part.vecs - (it * kLpWarps + warp) * kLpTurn));
+  };
+  auto fetch = [&](int it, int slot) {
+    const int n = vectors(it);
+    if (n == 0) return;
+    mbar_arrive_expect_tx(&sh.full[warp][slot], n * 16);
+    bulk_g2s(sh.ring[warp][slot],
+             part.x + part.e0 + part.head + 4LL * (it * kLpWarps + warp) * kLpTurn, n * 16,
+             &sh.full[warp][slot]);
+  };
+  if (lane == 0) {
+    for (int i = 0; i < kLpStages; ++i) mbar_init(&sh.full[warp][i], 1);
+    fence_mbar_init();
+    for (int i = 0; i < kLpStages && i < turns; ++i) fetch(i, i);
+  }
   long long token = -1;
   float token_logit = 0.0f;
   if (a.tokens && rank == 0 && tid == 0) {
     token = a.tokens[row];
-    if (token >= 0 && token < a.vocab) token_logit = __ldg(x + token);
+    if (token >= 0 && token < a.vocab) token_logit = __ldg(part.x + token);
   }
-  // 16-byte vectors from the boundary at or before the row's first element, of
-  // which `skip` elements are not the row's
-  const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
-  const float* base = x - skip;
-  const long long end = static_cast<long long>(a.vocab) + skip;  // in elements of base
-  const int vecs = static_cast<int>((end + 3) >> 2);
-  const int first = static_cast<int>(static_cast<long long>(vecs) * rank / splits);
-  const int last = static_cast<int>(static_cast<long long>(vecs) * (rank + 1) / splits);
-  auto load = [&](int seg, float (&v)[kLpPer]) {
+  if (tid == 0) {
+    sh.count = 0;
+    sh.over = 0;
+    sh.floor = 0;
+  }
+  __syncthreads();
+  // The warp's maximum so far, and sums that refer to it and leave one instance of
+  // it out, in the lane whose n is 1.
+  float m = -INFINITY, n = 0.0f;
+  float2 s2 = make_float2(0.0f, 0.0f), w2 = make_float2(0.0f, 0.0f);
+  int cut = 1;  // the list is cut after this many turns
+#pragma unroll 1
+  for (int it = 0, slot = 0, phase = 0; it < all_turns; ++it) {
+    float v[kLpPer];
+    const int here = it < turns ? vectors(it) : 0;
+    if (here == kLpTurn) {
+      mbar_wait_try(&sh.full[warp][slot], phase, a.status);
 #pragma unroll
-    for (int r = 0; r < kLpVec; ++r) {
-      const int i = seg + r * kLpThreads + tid;
-      if (i < last && (i > 0 || skip == 0) && 4LL * i + 4 <= end) {
-        const float4 q = __ldcs(reinterpret_cast<const float4*>(base) + i);
+      for (int r = 0; r < kLpVec; ++r) {
+        const float4 q = sh.ring[warp][slot][r * 32 + lane];
         v[4 * r] = q.x;
         v[4 * r + 1] = q.y;
         v[4 * r + 2] = q.z;
         v[4 * r + 3] = q.w;
-      } else {
+      }
+    } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const long long e = 4LL * i + c;
-          v[4 * r + c] = i < last && e >= skip && e < end ? __ldcs(base + e) : -INFINITY;
-        }
+      for (int i = 0; i < kLpPer; ++i) v[i] = -INFINITY;
+      if (here > 0) {
+        mbar_wait_try(&sh.full[warp][slot], phase, a.status);
+#pragma unroll
+        for (int r = 0; r < kLpVec; ++r)
+          if (r * 32 + lane < here) {
+            const float4 q = sh.ring[warp][slot][r * 32 + lane];
+            v[4 * r] = q.x;
+            v[4 * r + 1] = q.y;
+            v[4 * r + 2] = q.z;
+            v[4 * r + 3] = q.w;
+          }
+      } else if (it >= turns && warp == 0 && lane < part.head + part.tail) {
+        v[0] = __ldg(part.x + part.index(it, turns, 0));
       }
     }
-  };
-  if (TOP) {
-    if (tid < 2) sh.count[tid] = 0;
-    if (tid == 0) sh.floor = 0;
-    __syncthreads();
-  }
-  float m = -INFINITY, s = 0.0f, w = 0.0f, n = 0.0f;
-  int cur = 0;  // the list in use
-  float v[kLpPer];
-  load(first, v);
-  for (int seg = first; seg < last; seg += kLpSegment) {
-    float next[kLpPer];
-    if (seg + kLpSegment < last) load(seg + kLpSegment, next);
+    __syncwarp();  // every lane has read the slot
+    if (lane == 0 && it + kLpStages < turns) fetch(it + kLpStages, slot);
+    if (++slot == kLpStages) {
+      slot = 0;
+      phase ^= 1;
+    }
     float mx = v[0];
 #pragma unroll
-    for (int i = 1; i < kLpPer; ++i) mx = fmaxf(mx, v[i]);
-    if (mx > m) {
-      lp_refer(m, mx, s, w, n);
-      m = mx;
-    }
-    const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-    for (int i = 0; i < kLpPer; ++i) {
-      const float z = v[i] - ref, e = lp_exp2(z * kLpLog2e);
-      if (z != 0.0f) s += e;  // NaN stays in the sum
-      else n += 1.0f;
-      w = fmaf(e, fmaxf(z, -1000.0f), w);
-    }
+    for (int i = 1; i + 1 < kLpPer; i += 2) mx = lp_max3(mx, v[i], v[i + 1]);
+    mx = fmaxf(mx, v[kLpPer - 1]);
     if (TOP) {
-      // the candidates of this segment
-      LpKey floor = sh.floor;
-      auto hits = [&] { return lp_order(mx) >= static_cast<uint32_t>(floor >> 32) && mx >= -INFINITY; };
-      // key of v[i], 0 where the segment has run out of this CTA's elements
-      auto key_of = [&](int i) {
-        const int at = seg + (i >> 2) * kLpThreads + tid, e = 4 * at + (i & 3) - skip;
-        return at < last && e >= 0 && e < a.vocab && !isnan(v[i]) ? lp_key(v[i], e) : 0;
-      };
-      const int before = sh.count[cur];  // (read ahead of the barrier: elements join behind it)
-      int threads = __syncthreads_count(hits());
-      if (threads) {
-        if (before + threads * kLpPer > kLpList) {
-          // a bound that k threads' maxima reach: the r-th best of every warp
-          uint32_t o = lp_order(mx), nth = 0;
-          for (int r = 0; r < (k + kLpWarps - 1) / kLpWarps; ++r) {
-            nth = __reduce_max_sync(0xffffffffu, o);
-            const unsigned who = __ballot_sync(0xffffffffu, o == nth);
-            if (lane == __ffs(who) - 1) o = 0;
-          }
-          if (lane == 0) sh.bound[warp] = nth;
-          __syncthreads();
-          uint32_t low = sh.bound[0];
+      if (it == 0) lp_bound(sh, lp_order(mx), k);
+      const float least = lp_logit(static_cast<uint32_t>(sh.floor >> 32));
+      if (__any_sync(0xffffffffu, mx >= least && mx > -INFINITY)) {
+        uint32_t hits = 0;
 #pragma unroll
-          for (int i = 1; i < kLpWarps; ++i) low = min(low, sh.bound[i]);
-          const LpKey at_least = static_cast<LpKey>(low) << 32;
-          floor = at_least > floor ? at_least : floor;
-          threads = __syncthreads_count(hits());
-        }
-        bool joins;
-        if (before + threads * kLpPer > kLpList) {
-          // still too many, as equal logits can be: the exact k-th best of the
-          // threads' best keys, which only k threads reach
-          if (before > kLpCut) {  // room first
-            lp_cut(sh, sh.list[cur], before, k, sh.list[cur ^ 1]);
-            __syncthreads();
-            if (tid == 0) sh.count[cur ^ 1] = k;
-            cur ^= 1;
-            __syncthreads();
-          }
-          LpKey best = 0;
-#pragma unroll
-          for (int i = 0; i < kLpPer; ++i) {
-            const LpKey key = key_of(i);
-            best = key > best ? key : best;
-          }
-          LpKey* keys = sh.list[cur ^ 1];
-          keys[tid] = best;
-          __syncthreads();
-          int above = 0;
-          for (int c = 0; c < kLpThreads; ++c) above += keys[c] > best;
-          if (above == k - 1 && best > floor) sh.floor = best;
-          __syncthreads();
-          floor = sh.floor > floor ? sh.floor : floor;
-          joins = best >= floor;
-          __syncthreads();  // everyone has read the floor and the keys
-        } else {
-          joins = hits();
-        }
-        if (joins) {
-#pragma unroll
-          for (int i = 0; i < kLpPer; ++i) {
-            const LpKey key = key_of(i);
-            if (key != 0 && key >= floor) {
-              const int at = atomicAdd(&sh.count[cur], 1);
-              if (at < kLpList) sh.list[cur][at] = key;
-            }
-          }
-        }
-        if (tid == 0 && floor > sh.floor) sh.floor = floor;
+        for (int i = 0; i < kLpPer; ++i) hits |= v[i] >= least && v[i] > -INFINITY ? 1u << i : 0u;
+        lp_join(sh, part, it, turns, hits);
+      }
+      if (it + 1 == cut) {
+        cut *= 4;
         __syncthreads();
-        const int held = min(sh.count[cur], kLpList);
-        if (held > k + 32) {
-          lp_cut(sh, sh.list[cur], held, k, sh.list[cur ^ 1]);
-          __syncthreads();
-          if (tid == 0) {
-            sh.count[cur ^ 1] = k;
-            sh.count[cur] = 0;
-          }
-          cur ^= 1;
-          __syncthreads();
+        const int held = sh.count;
+        __syncthreads();
+        if (held > kLpList) {
+          if (tid == 0) sh.over = 1;
+          cut = 0;  // the second pass picks: joins are only counted now
+        } else if (held > k) {
+          lp_cut(sh, held, k);
+        }
+        __syncthreads();
+      }
+    }
+    if (__any_sync(0xffffffffu, mx > m)) {
+      // a new maximum of the warp: the old one joins its lane's sums, one instance
+      // of the new one leaves
+      const float top = warp_max(mx > m ? mx : m);
+      float s = s2.x + s2.y, w = w2.x + w2.y;
+      lp_refer(m, top, s, w, n);
+      s2 = make_float2(s, 0.0f);
+      w2 = make_float2(w, 0.0f);
+      m = top;
+      const unsigned who = __ballot_sync(0xffffffffu, mx == m);
+      if (lane == __ffs(who) - 1) {
+        n = 1.0f;
+        bool left = false;
+#pragma unroll
+        for (int i = 0; i < kLpPer; ++i) {
+          const bool it_is = !left && v[i] == mx;
+          left |= it_is;
+          v[i] = it_is ? -INFINITY : v[i];
         }
       }
     }
+    const float ref = m == -INFINITY ? 0.0f : -m;
 #pragma unroll
-    for (int i = 0; i < kLpPer; ++i) v[i] = next[i];
+    for (int i = 0; i < kLpPer; i += 2) {
+      // z from -1000 up (e^z is 0 there, and e^z z is 0 too, not NaN); NaN stays
+      float2 z = f2_add(make_float2(v[i], v[i + 1]), make_float2(ref, ref));
+      z = make_float2(lp_max_nan(z.x, -1000.0f), lp_max_nan(z.y, -1000.0f));
+      const float2 y = f2_mul(z, make_float2(kLpLog2e, kLpLog2e));
+      const float2 e = make_float2(lp_exp2(y.x), lp_exp2(y.y));
+      s2 = f2_add(s2, e);
+      w2 = f2_fma(e, z, w2);
+    }
   }
+  float s = s2.x + s2.y, w = w2.x + w2.y;
 
   // ---- the CTA's sums, and its k best in order
-  const float wm = warp_max(m);
-  if (lane == 0) sh.m[warp] = wm;
+  if (lane == 0) sh.m[warp] = m;
   __syncthreads();
   float M = sh.m[0];
 #pragma unroll
@@ -282,9 +425,15 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     sh.n[warp] = n;
   }
   int held = 0;
-  if (TOP) {
-    held = min(sh.count[cur], kLpList);
-    lp_cut(sh, sh.list[cur], held, k, sh.list[cur ^ 1]);
+  if (TOP) {  // (every join lies behind the barrier above)
+    held = sh.count;
+    // the list has run full, or k logits that are not -inf have not been found
+    if (sh.over || held > kLpList || (held < k && held < part.e1 - part.e0)) {
+      __syncthreads();
+      lp_pick_exactly(sh, part, k);
+      held = sh.count;
+    }
+    lp_rank(sh, sh.list, held, k);
   }
   __syncthreads();
   s = w = n = 0.0f;
@@ -294,9 +443,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     w += sh.w[i];
     n += sh.n[i];
   }
-  const LpKey* ranked = sh.list[cur ^ 1];
   if (splits > 1) {
-    if (tid < k) sh.best[tid] = tid < held ? ranked[tid] : 0;
+    if (tid >= held && tid < k) sh.best[tid] = 0;
     if (tid == 0) {
       sh.part[0] = M;
       sh.part[1] = s;
@@ -307,25 +455,43 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (rank == 0) {
       const bool mine = lane < splits;
-      float pm = mine ? lp_remote(&sh.part[0], lane) : -INFINITY;
+      const float pm = mine ? lp_remote(&sh.part[0], lane) : -INFINITY;
       s = mine ? lp_remote(&sh.part[1], lane) : 0.0f;
       w = mine ? lp_remote(&sh.part[2], lane) : 0.0f;
       n = mine ? lp_remote(&sh.part[3], lane) : 0.0f;
+      // the parts' lists are in order (0 behind their ends: never among the k best
+      // of a row of k logits): a key's rank is its own place and, by bisection,
+      // the number of larger ones in every other list
+      const int all = splits * k, list = TOP ? tid / k : 0, place = tid - list * k;
+      LpKey* keys = sh.keys;
+      LpKey key = 0;
+      if (TOP && tid < all) keys[tid] = key = lp_remote(&sh.best[place], list);
       M = warp_max(pm);
       lp_refer(pm, M, s, w, n);
       s = warp_sum(s);
       w = warp_sum(w);
       n = warp_sum(n);
       if (TOP) {
-        // (0 stands for no key: it is never among the k best of a row of k logits)
-        const int all = splits * k;
-        LpKey key = 0;
-        if (tid < all) key = lp_remote(&sh.best[tid % k], tid / k);
-        LpKey* keys = sh.list[cur];
-        if (tid < all) keys[tid] = key;
-        held = all;
         __syncthreads();
-        lp_cut(sh, keys, all, k, sh.list[cur ^ 1]);
+        if (tid < all && key != 0) {
+          int larger[kLpCluster];
+#pragma unroll
+          for (int o = 0; o < kLpCluster; ++o) larger[o] = 0;
+#pragma unroll
+          for (int step = kLogprobMaxTop / 2; step > 0; step >>= 1)
+#pragma unroll
+            for (int o = 0; o < kLpCluster; ++o)
+              if (o < splits && larger[o] + step <= k && keys[o * k + larger[o] + step - 1] > key)
+                larger[o] += step;
+          int rank_of = place;
+#pragma unroll
+          for (int o = 0; o < kLpCluster; ++o)
+            if (o < splits && o != list) {
+              if (larger[o] < k && keys[o * k + larger[o]] > key) ++larger[o];
+              rank_of += larger[o];
+            }
+          if (rank_of < k) sh.list[rank_of] = key;
+        }
         __syncthreads();
       }
     }
@@ -344,7 +510,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
       }
     }
     if (TOP && tid < k) {
-      const LpKey key = ranked[tid];
+      const LpKey key = splits > 1 ? sh.list[tid] : sh.best[tid];
       const long long o = static_cast<long long>(row) * k + tid;
       a.top_ids[o] = bad ? -1 : lp_index(key);
       a.top_logprobs[o] = bad ? nan : (lp_logit(static_cast<uint32_t>(key >> 32)) - M) - lse;
@@ -357,26 +523,42 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
 }
 
 cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t st) {
-  // CTAs per row: while all are resident at once (four per SM) and each has a
-  // segment of its own
+  constexpr size_t smem = sizeof(LpShared);
+  static PerDeviceOnce configured;
+  configured.run([] {
+    cudaFuncSetAttribute(token_logprobs_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         static_cast<int>(smem));
+    cudaFuncSetAttribute(token_logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         static_cast<int>(smem));
+  });
+  // CTAs per row: while all are resident at once (three per SM) and each has a
+  // full ring
   a.splits = 1;
-  while (a.splits < kLpCluster && 2LL * rows * a.splits <= 4LL * sms &&
-         a.vocab > 4LL * kLpSegment * a.splits)
+  while (a.splits < kLpCluster && 2LL * rows * a.splits <= 3LL * sms &&
+         a.vocab > 4LL * kLpTurn * kLpWarps * a.splits)
     a.splits *= 2;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {static_cast<unsigned>(a.splits), 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(kLpThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
   constexpr int kMost = 1 << 27;  // rows of one launch (a grid holds 2^31 - 1 CTAs)
   for (int done = 0; done < rows; done += kMost) {
     const int now = rows - done < kMost ? rows - done : kMost;
     cfg.gridDim = dim3(static_cast<unsigned>(now) * a.splits);
-    const cudaError_t e = a.top_k ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<true>, a)
-                                  : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<false>, a);
+    auto kernel = a.top_k ? token_logprobs_kernel<true> : token_logprobs_kernel<false>;
+    cfg.numAttrs = 2;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e != cudaSuccess) {  // without the early start
+      cudaGetLastError();
+      cfg.numAttrs = 1;
+      e = cudaLaunchKernelEx(&cfg, kernel, a);
+    }
     if (e != cudaSuccess) return e;
     if (rows - done <= kMost) break;
     a.logits += now * a.ld;
