@@ -33,8 +33,10 @@ constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpVec = 4;                    // 16-byte vectors per lane and turn
 constexpr int kLpPer = 4 * kLpVec;           // elements per lane and turn
 constexpr int kLpTurn = 32 * kLpVec;         // vectors per warp and turn: one bulk copy
-constexpr int kLpStages = 3;                 // ring slots per warp
+constexpr int kLpStages = 2;                 // ring slots per warp
 constexpr int kLpCluster = 8;                // most CTAs per row (portable)
+// CTAs of no more turns than this look for candidates once, behind the loop.
+constexpr int kLpLate = 8;
 // Candidates: at most kLpCut stay after a cut, kLogprobMaxTop threads' elements
 // join by the exact bound.
 constexpr int kLpList = 1024;
@@ -57,6 +59,10 @@ __device__ __forceinline__ int lp_index(LpKey key) {
 __device__ __forceinline__ float lp_logit(uint32_t order) {
   return __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
 }
+// The logit that a candidate reaches: the floor's, but never -inf.
+__device__ __forceinline__ float lp_least(LpKey floor) {
+  return fmaxf(lp_logit(static_cast<uint32_t>(floor >> 32)), -3.402823466e38f);
+}
 
 __device__ __forceinline__ float lp_exp2(float x) {  // 2 ulp
   float y;
@@ -66,35 +72,36 @@ __device__ __forceinline__ float lp_exp2(float x) {  // 2 ulp
 
 struct LpShared {
   alignas(128) float4 ring[kLpWarps][kLpStages][kLpTurn];
-  alignas(16) LpKey list[kLpList];
-  alignas(16) LpKey keys[kLpThreads];        // the threads' best; the parts' lists of a row
+  alignas(16) LpKey list[kLpList + 8];       // zeros up to a multiple of eight when ranked
+  alignas(16) LpKey keys[kLpThreads];        // the threads' best
   LpKey best[kLogprobMaxTop];                // the k best of a cut, in order
   LpKey floor;
   uint64_t full[kLpWarps][kLpStages];
   float m[kLpWarps], s[kLpWarps], w[kLpWarps], n[kLpWarps];
   float part[4];                             // the CTA's {M, S, W, n}
   uint32_t bound[kLpWarps];
+  float best_of[kLpLate][kLpThreads];        // the threads' maxima turn by turn
   int count;                                 // candidates that have joined
   int over;                                  // more than the list holds
 };
 
-// The k best of src[0, n), in order, into sh.best; the k-th best, where there
+// The k best of the list's n, in order, into sh.best; the k-th best, where there
 // are k, is the new floor.  All threads; a barrier before and after.
-__device__ __forceinline__ void lp_rank(LpShared& sh, const LpKey* src, int n, int k) {
+__device__ __noinline__ void lp_rank(LpShared& sh, int n, int k) {
+  if (threadIdx.x < 8) sh.list[n + threadIdx.x] = 0;
+  __syncthreads();
 #pragma unroll 1
   for (int i = threadIdx.x; i < n; i += kLpThreads) {
-    const LpKey mine = src[i];
-    int rank = 0, c = 0;
+    const LpKey mine = sh.list[i];
+    int rank = 0;
 #pragma unroll 1
-    for (; c + 8 <= n; c += 8) {
+    for (int c = 0; c < n; c += 8) {
       ulonglong2 o[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) o[u] = *reinterpret_cast<const ulonglong2*>(src + c + 2 * u);
+      for (int u = 0; u < 4; ++u) o[u] = *reinterpret_cast<const ulonglong2*>(sh.list + c + 2 * u);
 #pragma unroll
       for (int u = 0; u < 4; ++u) rank += (o[u].x > mine) + (o[u].y > mine);
     }
-#pragma unroll 1
-    for (; c < n; ++c) rank += src[c] > mine;
     if (rank < k) sh.best[rank] = mine;
     if (rank == k - 1) sh.floor = mine;
   }
@@ -102,7 +109,7 @@ __device__ __forceinline__ void lp_rank(LpShared& sh, const LpKey* src, int n, i
 
 // The list cut back to its k best (n > k of them).  All threads, between barriers.
 __device__ __noinline__ void lp_cut(LpShared& sh, int n, int k) {
-  lp_rank(sh, sh.list, n, k);
+  lp_rank(sh, n, k);
   __syncthreads();
   if (threadIdx.x < k) sh.list[threadIdx.x] = sh.best[threadIdx.x];
   if (threadIdx.x == 0) sh.count = k;
@@ -163,9 +170,11 @@ struct LpRow {
 };
 
 // The hits of a turn (bits: elements of this lane) join the list: one place per
-// warp, its lanes' elements next to each other.  Their logits are read again: a
-// rare call with as little code in the loop as can be.
-__device__ __noinline__ void lp_join(LpShared& sh, const LpRow& row, int it, int turns, uint32_t hits) {
+// warp, its lanes' elements next to each other.  Their logits are read again from
+// the ring's slot: a rare call, with as little code in the loop as can be (with
+// this unrolled over the registers the loop outgrew the instruction cache).
+__device__ __noinline__ void lp_join(LpShared& sh, const LpRow& row, int it, int turns, uint32_t hits,
+                                     const float4* slot) {
   const int lane = threadIdx.x & 31, mine = __popc(hits);
   int upto = mine;
 #pragma unroll
@@ -178,8 +187,10 @@ __device__ __noinline__ void lp_join(LpShared& sh, const LpRow& row, int it, int
   at = __shfl_sync(0xffffffffu, at, 31) + upto - mine;
 #pragma unroll 1
   for (; hits; hits &= hits - 1, ++at) {
-    const int e = row.index(it, turns, __ffs(hits) - 1);
-    if (at < kLpList) sh.list[at] = lp_key(__ldg(row.x + e), e);
+    const int i = __ffs(hits) - 1, e = row.index(it, turns, i);
+    const float v = it < turns ? reinterpret_cast<const float*>(slot + (i >> 2) * 32 + lane)[i & 3]
+                               : __ldg(row.x + e);
+    if (at < kLpList) sh.list[at] = lp_key(v, e);
   }
 }
 
@@ -202,6 +213,44 @@ __device__ __noinline__ void lp_bound(LpShared& sh, uint32_t order, int k) {
     sh.floor = static_cast<LpKey>(low) << 32;
   }
   __syncthreads();
+}
+
+// The elements of this lane that reach `least` join the list, read again (from
+// L2) in the turns whose maximum of the lane does.  Code that runs once per
+// launch is rolled up: fetching it costs more than running it.
+__device__ __noinline__ void lp_join_late(LpShared& sh, const LpRow& row, int turns, int all_turns,
+                                          float least) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t todo = 0;
+#pragma unroll
+  for (int it = 0; it < kLpLate; ++it)
+    if (it < all_turns && sh.best_of[it][threadIdx.x] >= least) todo |= 1u << it;
+#pragma unroll 1
+  for (; todo; todo &= todo - 1) {
+    const int it = __ffs(todo) - 1;
+    uint32_t hits = 0;
+    if (it < turns) {
+      const float4* vec = reinterpret_cast<const float4*>(row.x + row.e0 + row.head);
+      float4 q[kLpVec];
+#pragma unroll
+      for (int r = 0; r < kLpVec; ++r) {
+        const int at = (it * kLpWarps + warp) * kLpTurn + r * 32 + lane;
+        q[r] = at < row.vecs ? __ldg(vec + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      }
+#pragma unroll
+      for (int r = 0; r < kLpVec; ++r)
+        hits |= ((q[r].x >= least ? 1u : 0u) | (q[r].y >= least ? 2u : 0u) | (q[r].z >= least ? 4u : 0u) |
+                 (q[r].w >= least ? 8u : 0u)) << (4 * r);
+    } else if (warp == 0 && lane < row.head + row.tail) {
+      hits = 1;
+    }
+#pragma unroll 1
+    for (; hits; hits &= hits - 1) {
+      const int e = row.index(it, turns, __ffs(hits) - 1);
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kLpList) sh.list[at] = lp_key(__ldg(row.x + e), e);
+    }
+  }
 }
 
 // The candidates of the CTA's elements picked again, whatever the logits are:
@@ -244,14 +293,14 @@ __device__ __noinline__ void lp_pick_exactly(LpShared& sh, const LpRow& row, int
     }
     __syncthreads();
     const int held = sh.count;
-    __syncthreads();
     if (held > kLpCut) lp_cut(sh, held, k);  // room for the next 4096's
+    __syncthreads();
   }
   __syncthreads();
 }
 
 template <bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LogprobArgs a) {
   extern __shared__ __align__(128) unsigned char lp_raw[];
   LpShared& sh = *reinterpret_cast<LpShared*>(lp_raw);
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
@@ -309,6 +358,8 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const Log
   float m = -INFINITY, n = 0.0f;
   float2 s2 = make_float2(0.0f, 0.0f), w2 = make_float2(0.0f, 0.0f);
   int cut = 1;  // the list is cut after this many turns
+  const bool late = all_turns <= kLpLate;
+  float best = -INFINITY;  // of this lane
 #pragma unroll 1
   for (int it = 0, slot = 0, phase = 0; it < all_turns; ++it) {
     float v[kLpPer];
@@ -341,37 +392,44 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const Log
         v[0] = __ldg(part.x + part.index(it, turns, 0));
       }
     }
+    float mx = v[0];
+#pragma unroll
+    for (int i = 1; i + 1 < kLpPer; i += 2) mx = lp_max3(mx, v[i], v[i + 1]);
+    mx = fmaxf(mx, v[kLpPer - 1]);
+    if (TOP && late) {
+      best = fmaxf(best, mx);
+      sh.best_of[it][tid] = mx;
+    } else if (TOP) {
+      if (it == 0) lp_bound(sh, lp_order(mx), k);
+      const float least = lp_least(sh.floor);
+      if (__any_sync(0xffffffffu, mx >= least)) {
+        uint32_t hits = 0;
+#pragma unroll
+        for (int i = 0; i < kLpPer; ++i) hits |= v[i] >= least ? 1u << i : 0u;
+        lp_join(sh, part, it, turns, hits, sh.ring[warp][slot]);
+      }
+    }
     __syncwarp();  // every lane has read the slot
     if (lane == 0 && it + kLpStages < turns) fetch(it + kLpStages, slot);
     if (++slot == kLpStages) {
       slot = 0;
       phase ^= 1;
     }
-    float mx = v[0];
-#pragma unroll
-    for (int i = 1; i + 1 < kLpPer; i += 2) mx = lp_max3(mx, v[i], v[i + 1]);
-    mx = fmaxf(mx, v[kLpPer - 1]);
-    if (TOP) {
-      if (it == 0) lp_bound(sh, lp_order(mx), k);
-      const float least = lp_logit(static_cast<uint32_t>(sh.floor >> 32));
-      if (__any_sync(0xffffffffu, mx >= least && mx > -INFINITY)) {
-        uint32_t hits = 0;
-#pragma unroll
-        for (int i = 0; i < kLpPer; ++i) hits |= v[i] >= least && v[i] > -INFINITY ? 1u << i : 0u;
-        lp_join(sh, part, it, turns, hits);
-      }
-      if (it + 1 == cut) {
+    if (TOP && !late) {
+      if (it + 1 == cut && it + 1 < all_turns) {
         cut *= 4;
         __syncthreads();
-        const int held = sh.count;
-        __syncthreads();
+        const int held = sh.count;  // (written next behind a barrier)
         if (held > kLpList) {
           if (tid == 0) sh.over = 1;
           cut = 0;  // the second pass picks: joins are only counted now
+          __syncthreads();
         } else if (held > k) {
           lp_cut(sh, held, k);
+          __syncthreads();
+        } else {
+          __syncthreads();
         }
-        __syncthreads();
       }
     }
     if (__any_sync(0xffffffffu, mx > m)) {
@@ -408,6 +466,10 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const Log
     }
   }
   float s = s2.x + s2.y, w = w2.x + w2.y;
+  if (TOP && late) {
+    lp_bound(sh, lp_order(best), k);
+    lp_join_late(sh, part, turns, all_turns, lp_least(sh.floor));
+  }
 
   // ---- the CTA's sums, and its k best in order
   if (lane == 0) sh.m[warp] = m;
@@ -433,7 +495,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const Log
       lp_pick_exactly(sh, part, k);
       held = sh.count;
     }
-    lp_rank(sh, sh.list, held, k);
+    lp_rank(sh, held, k);
   }
   __syncthreads();
   s = w = n = 0.0f;
@@ -459,39 +521,27 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const Log
       s = mine ? lp_remote(&sh.part[1], lane) : 0.0f;
       w = mine ? lp_remote(&sh.part[2], lane) : 0.0f;
       n = mine ? lp_remote(&sh.part[3], lane) : 0.0f;
-      // the parts' lists are in order (0 behind their ends: never among the k best
-      // of a row of k logits): a key's rank is its own place and, by bisection,
-      // the number of larger ones in every other list
-      const int all = splits * k, list = TOP ? tid / k : 0, place = tid - list * k;
-      LpKey* keys = sh.keys;
+      // the parts' k best (0 behind their ends: never among those of a row of k logits)
+      const int all = splits * k;
       LpKey key = 0;
-      if (TOP && tid < all) keys[tid] = key = lp_remote(&sh.best[place], list);
-      M = warp_max(pm);
+      if (TOP && tid < all) key = lp_remote(&sh.best[tid % k], tid / k);
+      M = pm;
+#pragma unroll
+      for (int o = 1; o < kLpCluster; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      M = __shfl_sync(0xffffffffu, M, 0);
       lp_refer(pm, M, s, w, n);
-      s = warp_sum(s);
-      w = warp_sum(w);
-      n = warp_sum(n);
+#pragma unroll
+      for (int o = 1; o < kLpCluster; o <<= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        w += __shfl_xor_sync(0xffffffffu, w, o);
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+      }
+      s = __shfl_sync(0xffffffffu, s, 0);
+      w = __shfl_sync(0xffffffffu, w, 0);
+      n = __shfl_sync(0xffffffffu, n, 0);
       if (TOP) {
-        __syncthreads();
-        if (tid < all && key != 0) {
-          int larger[kLpCluster];
-#pragma unroll
-          for (int o = 0; o < kLpCluster; ++o) larger[o] = 0;
-#pragma unroll
-          for (int step = kLogprobMaxTop / 2; step > 0; step >>= 1)
-#pragma unroll
-            for (int o = 0; o < kLpCluster; ++o)
-              if (o < splits && larger[o] + step <= k && keys[o * k + larger[o] + step - 1] > key)
-                larger[o] += step;
-          int rank_of = place;
-#pragma unroll
-          for (int o = 0; o < kLpCluster; ++o)
-            if (o < splits && o != list) {
-              if (larger[o] < k && keys[o * k + larger[o]] > key) ++larger[o];
-              rank_of += larger[o];
-            }
-          if (rank_of < k) sh.list[rank_of] = key;
-        }
+        if (tid < all) sh.list[tid] = key;
+        lp_rank(sh, all, k);
         __syncthreads();
       }
     }
@@ -510,7 +560,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(const Log
       }
     }
     if (TOP && tid < k) {
-      const LpKey key = splits > 1 ? sh.list[tid] : sh.best[tid];
+      const LpKey key = sh.best[tid];
       const long long o = static_cast<long long>(row) * k + tid;
       a.top_ids[o] = bad ? -1 : lp_index(key);
       a.top_logprobs[o] = bad ? nan : (lp_logit(static_cast<uint32_t>(key >> 32)) - M) - lse;
@@ -531,10 +581,10 @@ cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t
     cudaFuncSetAttribute(token_logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          static_cast<int>(smem));
   });
-  // CTAs per row: while all are resident at once (three per SM) and each has a
+  // CTAs per row: while all are resident at once (four per SM) and each has a
   // full ring
   a.splits = 1;
-  while (a.splits < kLpCluster && 2LL * rows * a.splits <= 3LL * sms &&
+  while (a.splits < kLpCluster && 2LL * rows * a.splits <= 4LL * sms &&
          a.vocab > 4LL * kLpTurn * kLpWarps * a.splits)
     a.splits *= 2;
   cudaLaunchAttribute attr[2];
