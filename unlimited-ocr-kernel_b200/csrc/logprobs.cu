@@ -10,17 +10,18 @@
 // precision, and both terms of H are >= 0, so nothing cancels.
 //
 // One pass: every warp keeps the maximum of what it has seen and sums that refer
-// to it; a new maximum, a rare thing, rescales them.  The alternatives come
-// from a short list of candidates per CTA: an element joins when its key (logit,
-// then lower index) reaches a bound that k keys are known to reach.  The first
-// bound comes from the first segment's threads' maxima, the next ones from
-// cutting the list back to its k best after segments 1, 4, 16, 64, ...; in
-// between no warp waits for another.  Where that list runs full (logits that
-// rise along the row, thousands of equal ones), or fewer than k logits are
-// finite, the alternatives are picked in a second pass that bounds every
-// segment exactly.  A row is spread over a cluster of CTAs where the rows are
-// few; the CTAs' sums and lists are joined through distributed shared memory.
+// to it; a new maximum, a rare thing, rescales them.  The alternatives cost the
+// loop one 16-bit store: every lane leaves the maximum of each of its turns.
+// Behind the loop (or 32 turns) k lanes' best logits give a bound that k elements
+// reach, the few turns whose maximum reaches it are read again, their elements
+// that do become a short list of candidates, and their rank in it gives the k
+// best.  Where the list runs full (thousands of equal logits), or fewer than k
+// logits are finite, a second pass bounds every 4096 elements exactly.  A row is
+// spread over a cluster of CTAs where the rows are few; the CTAs' sums and lists
+// are joined through distributed shared memory.
 #include <cuda_runtime.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "device_once.h"
@@ -35,11 +36,10 @@ constexpr int kLpPer = 4 * kLpVec;           // elements per lane and turn
 constexpr int kLpTurn = 32 * kLpVec;         // vectors per warp and turn: one bulk copy
 constexpr int kLpStages = 2;                 // ring slots per warp
 constexpr int kLpCluster = 8;                // most CTAs per row (portable)
-// CTAs of no more turns than this look for candidates once, behind the loop.
-constexpr int kLpLate = 8;
+constexpr int kLpKept = 32;                  // turns whose maxima are kept
 // Candidates: at most kLpCut stay after a cut, kLogprobMaxTop threads' elements
 // join by the exact bound.
-constexpr int kLpList = 1024;
+constexpr int kLpList = 768;
 constexpr int kLpCut = kLpList - kLogprobMaxTop * kLpPer;
 constexpr float kLpLog2e = 1.44269504f;
 
@@ -59,6 +59,14 @@ __device__ __forceinline__ int lp_index(LpKey key) {
 __device__ __forceinline__ float lp_logit(uint32_t order) {
   return __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order);
 }
+// The upper half of the smallest bf16 >= x, and back.
+__device__ __forceinline__ uint16_t lp_up16(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return static_cast<uint16_t>((u & 0x80000000u ? u : u + 0xFFFFu) >> 16);
+}
+__device__ __forceinline__ float lp_from16(uint16_t h) {
+  return __uint_as_float(static_cast<uint32_t>(h) << 16);
+}
 // The logit that a candidate reaches: the floor's, but never -inf.
 __device__ __forceinline__ float lp_least(LpKey floor) {
   return fmaxf(lp_logit(static_cast<uint32_t>(floor >> 32)), -3.402823466e38f);
@@ -73,14 +81,13 @@ __device__ __forceinline__ float lp_exp2(float x) {  // 2 ulp
 struct LpShared {
   alignas(128) float4 ring[kLpWarps][kLpStages][kLpTurn];
   alignas(16) LpKey list[kLpList + 8];       // zeros up to a multiple of eight when ranked
-  alignas(16) LpKey keys[kLpThreads];        // the threads' best
+  uint16_t kept[kLpKept][kLpThreads];        // the lanes' maxima turn by turn (lp_up16)
   LpKey best[kLogprobMaxTop];                // the k best of a cut, in order
   LpKey floor;
   uint64_t full[kLpWarps][kLpStages];
   float m[kLpWarps], s[kLpWarps], w[kLpWarps], n[kLpWarps];
   float part[4];                             // the CTA's {M, S, W, n}
   uint32_t bound[kLpWarps];
-  float best_of[kLpLate][kLpThreads];        // the threads' maxima turn by turn
   int count;                                 // candidates that have joined
   int over;                                  // more than the list holds
 };
@@ -165,34 +172,20 @@ struct LpRow {
   __device__ __forceinline__ int index(int it, int turns, int i) const {
     const int lane = threadIdx.x & 31;
     if (it >= turns) return lane < head ? e0 + lane : e1 - tail + lane - head;
-    return e0 + head + 4 * ((it * kLpWarps + (threadIdx.x >> 5)) * kLpTurn + (i >> 2) * 32 + lane) + (i & 3);
+    return e0 + head + 4 * (start(it, turns) + (i >> 2) * 32 + lane) + (i & 3);
+  }
+  // Vectors of each warp's turn: the last turn's are shared out evenly.
+  __device__ __forceinline__ int share(int it, int turns) const {
+    return it == turns - 1 ? (vecs - it * kLpWarps * kLpTurn + kLpWarps - 1) / kLpWarps : kLpTurn;
+  }
+  // This warp's first, and how many.
+  __device__ __forceinline__ int start(int it, int turns) const {
+    return it * kLpWarps * kLpTurn + static_cast<int>(threadIdx.x >> 5) * share(it, turns);
+  }
+  __device__ __forceinline__ int count(int it, int turns) const {
+    return max(0, min(share(it, turns), vecs - start(it, turns)));
   }
 };
-
-// The hits of a turn (bits: elements of this lane) join the list: one place per
-// warp, its lanes' elements next to each other.  Their logits are read again from
-// the ring's slot: a rare call, with as little code in the loop as can be (with
-// this unrolled over the registers the loop outgrew the instruction cache).
-__device__ __noinline__ void lp_join(LpShared& sh, const LpRow& row, int it, int turns, uint32_t hits,
-                                     const float4* slot) {
-  const int lane = threadIdx.x & 31, mine = __popc(hits);
-  int upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int below = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += below;
-  }
-  int at = 0;
-  if (lane == 31) at = atomicAdd(&sh.count, upto);
-  at = __shfl_sync(0xffffffffu, at, 31) + upto - mine;
-#pragma unroll 1
-  for (; hits; hits &= hits - 1, ++at) {
-    const int i = __ffs(hits) - 1, e = row.index(it, turns, i);
-    const float v = it < turns ? reinterpret_cast<const float*>(slot + (i >> 2) * 32 + lane)[i & 3]
-                               : __ldg(row.x + e);
-    if (at < kLpList) sh.list[at] = lp_key(v, e);
-  }
-}
 
 // The r-th best of every warp's 32 orders, r = ceil(k / warps): k threads reach
 // the least of them, and so do k elements.  A barrier before and after.
@@ -210,32 +203,34 @@ __device__ __noinline__ void lp_bound(LpShared& sh, uint32_t order, int k) {
     uint32_t low = sh.bound[0];
 #pragma unroll
     for (int i = 1; i < kLpWarps; ++i) low = min(low, sh.bound[i]);
-    sh.floor = static_cast<LpKey>(low) << 32;
+    const LpKey floor = static_cast<LpKey>(low) << 32;
+    if (floor > sh.floor) sh.floor = floor;
   }
   __syncthreads();
 }
 
-// The elements of this lane that reach `least` join the list, read again (from
-// L2) in the turns whose maximum of the lane does.  Code that runs once per
-// launch is rolled up: fetching it costs more than running it.
-__device__ __noinline__ void lp_join_late(LpShared& sh, const LpRow& row, int turns, int all_turns,
-                                          float least) {
+// The elements of this lane's turns [from, to) that reach `least` join the list:
+// read again (usually from L2) in the turns whose maximum does.  Code that runs
+// once per launch is rolled up: fetching it costs more than running it.
+__device__ __noinline__ void lp_join(LpShared& sh, const LpRow& row, int turns, int from, int to,
+                                     float least) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t todo = 0;
-#pragma unroll
-  for (int it = 0; it < kLpLate; ++it)
-    if (it < all_turns && sh.best_of[it][threadIdx.x] >= least) todo |= 1u << it;
+#pragma unroll 8
+  for (int i = 0; i < to - from; ++i)
+    if (lp_from16(sh.kept[i][threadIdx.x]) >= least) todo |= 1u << i;
 #pragma unroll 1
   for (; todo; todo &= todo - 1) {
-    const int it = __ffs(todo) - 1;
+    const int it = from + __ffs(todo) - 1;
     uint32_t hits = 0;
     if (it < turns) {
       const float4* vec = reinterpret_cast<const float4*>(row.x + row.e0 + row.head);
       float4 q[kLpVec];
 #pragma unroll
       for (int r = 0; r < kLpVec; ++r) {
-        const int at = (it * kLpWarps + warp) * kLpTurn + r * 32 + lane;
-        q[r] = at < row.vecs ? __ldg(vec + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        q[r] = r * 32 + lane < row.count(it, turns)
+                   ? __ldg(vec + row.start(it, turns) + r * 32 + lane)
+                   : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       }
 #pragma unroll
       for (int r = 0; r < kLpVec; ++r)
@@ -258,6 +253,7 @@ __device__ __noinline__ void lp_join_late(LpShared& sh, const LpRow& row, int tu
 // only k threads reach.  The list ends with all of the k best in it.
 __device__ __noinline__ void lp_pick_exactly(LpShared& sh, const LpRow& row, int k) {
   const int tid = threadIdx.x;
+  LpKey* keys = reinterpret_cast<LpKey*>(sh.ring);  // (every copy has landed and been read)
   if (tid == 0) sh.count = 0;
 #pragma unroll 1
   for (int first = row.e0; first < row.e1; first += kLpThreads * kLpPer) {
@@ -270,12 +266,12 @@ __device__ __noinline__ void lp_pick_exactly(LpShared& sh, const LpRow& row, int
       best = key > best ? key : best;
     }
     __syncthreads();
-    sh.keys[tid] = best;
+    keys[tid] = best;
     __syncthreads();
     int above = 0;
 #pragma unroll 4
     for (int c = 0; c < kLpThreads; c += 2) {
-      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(sh.keys + c);
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(keys + c);
       above += (o.x > best) + (o.y > best);
     }
     if (above == k - 1 && best > sh.floor) sh.floor = best;  // (one thread, the only reader)
@@ -325,15 +321,12 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   // the elements at the ends
   const int turns = (part.vecs + kLpWarps * kLpTurn - 1) / (kLpWarps * kLpTurn);
   const int all_turns = turns + (part.head + part.tail > 0);
-  auto vectors = [&](int it) {  // of this warp's turn
-    return max(0, min(kLpTurn, part.vecs - (it * kLpWarps + warp) * kLpTurn));
-  };
   auto fetch = [&](int it, int slot) {
-    const int n = vectors(it);
+    const int n = part.count(it, turns);
     if (n == 0) return;
     mbar_arrive_expect_tx(&sh.full[warp][slot], n * 16);
     bulk_g2s(sh.ring[warp][slot],
-             part.x + part.e0 + part.head + 4LL * (it * kLpWarps + warp) * kLpTurn, n * 16,
+             part.x + part.e0 + part.head + 4LL * part.start(it, turns), n * 16,
              &sh.full[warp][slot]);
   };
   if (lane == 0) {
@@ -357,13 +350,18 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   // it out, in the lane whose n is 1.
   float m = -INFINITY, n = 0.0f;
   float2 s2 = make_float2(0.0f, 0.0f), w2 = make_float2(0.0f, 0.0f);
-  int cut = 1;  // the list is cut after this many turns
-  const bool late = all_turns <= kLpLate;
-  float best = -INFINITY;  // of this lane
+  float best = -INFINITY;  // of this lane, since turn `from`
+  int from = 0;
+  // the candidates of turns [from, to)
+  auto gather = [&](int to) {
+    lp_bound(sh, lp_order(best), k);
+    lp_join(sh, part, turns, from, to, lp_least(sh.floor));
+    __syncthreads();
+  };
 #pragma unroll 1
   for (int it = 0, slot = 0, phase = 0; it < all_turns; ++it) {
     float v[kLpPer];
-    const int here = it < turns ? vectors(it) : 0;
+    const int here = it < turns ? part.count(it, turns) : 0;
     if (here == kLpTurn) {
       mbar_wait_try(&sh.full[warp][slot], phase, a.status);
 #pragma unroll
@@ -396,41 +394,15 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
 #pragma unroll
     for (int i = 1; i + 1 < kLpPer; i += 2) mx = lp_max3(mx, v[i], v[i + 1]);
     mx = fmaxf(mx, v[kLpPer - 1]);
-    if (TOP && late) {
+    if (TOP) {
       best = fmaxf(best, mx);
-      sh.best_of[it][tid] = mx;
-    } else if (TOP) {
-      if (it == 0) lp_bound(sh, lp_order(mx), k);
-      const float least = lp_least(sh.floor);
-      if (__any_sync(0xffffffffu, mx >= least)) {
-        uint32_t hits = 0;
-#pragma unroll
-        for (int i = 0; i < kLpPer; ++i) hits |= v[i] >= least ? 1u << i : 0u;
-        lp_join(sh, part, it, turns, hits, sh.ring[warp][slot]);
-      }
+      sh.kept[it - from][tid] = lp_up16(mx);
     }
     __syncwarp();  // every lane has read the slot
     if (lane == 0 && it + kLpStages < turns) fetch(it + kLpStages, slot);
     if (++slot == kLpStages) {
       slot = 0;
       phase ^= 1;
-    }
-    if (TOP && !late) {
-      if (it + 1 == cut && it + 1 < all_turns) {
-        cut *= 4;
-        __syncthreads();
-        const int held = sh.count;  // (written next behind a barrier)
-        if (held > kLpList) {
-          if (tid == 0) sh.over = 1;
-          cut = 0;  // the second pass picks: joins are only counted now
-          __syncthreads();
-        } else if (held > k) {
-          lp_cut(sh, held, k);
-          __syncthreads();
-        } else {
-          __syncthreads();
-        }
-      }
     }
     if (__any_sync(0xffffffffu, mx > m)) {
       // a new maximum of the warp: the old one joins its lane's sums, one instance
@@ -464,12 +436,22 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
       s2 = f2_add(s2, e);
       w2 = f2_fma(e, z, w2);
     }
+    if (TOP && it + 1 - from == kLpKept && it + 1 < all_turns) {
+      gather(it + 1);
+      const int held = sh.count;  // (written next behind a barrier)
+      if (held > kLpList) {
+        if (tid == 0) sh.over = 1;
+      } else if (held > kLpCut) {
+        lp_cut(sh, held, k);
+      }
+      __syncthreads();
+      if (tid == 0 && held > kLpList) sh.count = 0;  // (the second pass will pick)
+      from = it + 1;
+      best = -INFINITY;
+    }
   }
   float s = s2.x + s2.y, w = w2.x + w2.y;
-  if (TOP && late) {
-    lp_bound(sh, lp_order(best), k);
-    lp_join_late(sh, part, turns, all_turns, lp_least(sh.floor));
-  }
+  if (TOP && all_turns) gather(all_turns);
 
   // ---- the CTA's sums, and its k best in order
   if (lane == 0) sh.m[warp] = m;
@@ -507,6 +489,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   }
   if (splits > 1) {
     if (tid >= held && tid < k) sh.best[tid] = 0;
+    if (tid == 0) sh.count = 0;
     if (tid == 0) {
       sh.part[0] = M;
       sh.part[1] = s;
@@ -521,10 +504,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
       s = mine ? lp_remote(&sh.part[1], lane) : 0.0f;
       w = mine ? lp_remote(&sh.part[2], lane) : 0.0f;
       n = mine ? lp_remote(&sh.part[3], lane) : 0.0f;
-      // the parts' k best (0 behind their ends: never among those of a row of k logits)
-      const int all = splits * k;
-      LpKey key = 0;
-      if (TOP && tid < all) key = lp_remote(&sh.best[tid % k], tid / k);
+      // the parts' k best (0 behind their ends: never among those of a row of k
+      // logits); k of them reach the least of the parts' r-th best, r = ceil(k / splits)
+      LpKey key = 0, least = ~0ull;
+      if (TOP && tid < splits * k) key = lp_remote(&sh.best[tid % k], tid / k);
+      if (TOP && mine) least = lp_remote(&sh.best[(k + splits - 1) / splits - 1], lane);
       M = pm;
 #pragma unroll
       for (int o = 1; o < kLpCluster; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
@@ -540,8 +524,15 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
       w = __shfl_sync(0xffffffffu, w, 0);
       n = __shfl_sync(0xffffffffu, n, 0);
       if (TOP) {
-        if (tid < all) sh.list[tid] = key;
-        lp_rank(sh, all, k);
+#pragma unroll
+        for (int o = 1; o < kLpCluster; o <<= 1) {
+          const LpKey other = __shfl_xor_sync(0xffffffffu, least, o);
+          least = other < least ? other : least;
+        }
+        least = __shfl_sync(0xffffffffu, least, 0);
+        if (key != 0 && key >= least) sh.list[atomicAdd(&sh.count, 1)] = key;
+        __syncthreads();
+        lp_rank(sh, sh.count, k);
         __syncthreads();
       }
     }
@@ -572,14 +563,35 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   }
 }
 
+// Clusters of `splits` CTAs that fit the device at once with `per` CTAs on an SM,
+// asked once per device (0 where the answer is an error).
+static int lp_clusters(int splits, int per, cudaLaunchConfig_t cfg) {
+  static std::atomic<int> known[64][9][5];  // answer + 1
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<int>* at = dev >= 0 && dev < 64 ? &known[dev][splits][per] : nullptr;
+  if (at && at->load(std::memory_order_relaxed)) return at->load(std::memory_order_relaxed) - 1;
+  int n = 0;
+  cfg.gridDim = dim3(splits);
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, token_logprobs_kernel<true>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (at) at->store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
 cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t st) {
   constexpr size_t smem = sizeof(LpShared);
+  constexpr int kLpSmemSm = 228 * 1024;  // of an SM, 1 KB of it the system's per CTA
+  static_assert(4 * (smem + 1024) <= kLpSmemSm, "four CTAs per SM");
   static PerDeviceOnce configured;
   configured.run([] {
     cudaFuncSetAttribute(token_logprobs_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         static_cast<int>(smem));
+                         kLpSmemSm / 2 - 1024);
     cudaFuncSetAttribute(token_logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         static_cast<int>(smem));
+                         kLpSmemSm / 2 - 1024);
   });
   // CTAs per row: while all are resident at once (four per SM) and each has a
   // full ring
@@ -594,9 +606,20 @@ cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(kLpThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
+  // Clusters are packed onto as few SMs as hold them: where two or three CTAs per
+  // SM hold all of them, a CTA asks for more shared memory than it uses, so that
+  // no more share one (150 rows of 129,280 logits: 34.4 -> 18.2 us).
+  cfg.dynamicSmemBytes = smem;
+  for (int per = 2; per < 4; ++per) {
+    cudaLaunchConfig_t wide = cfg;
+    wide.dynamicSmemBytes = kLpSmemSm / per - 1024;
+    if (lp_clusters(a.splits, per, wide) >= rows) {
+      cfg.dynamicSmemBytes = wide.dynamicSmemBytes;
+      break;
+    }
+  }
   constexpr int kMost = 1 << 27;  // rows of one launch (a grid holds 2^31 - 1 CTAs)
   for (int done = 0; done < rows; done += kMost) {
     const int now = rows - done < kMost ? rows - done : kMost;
