@@ -593,10 +593,11 @@ cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t
     cudaFuncSetAttribute(token_logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          kLpSmemSm / 2 - 1024);
   });
-  // CTAs per row: while all are resident at once (four per SM) and each has a
-  // full ring
+  // CTAs per row: while three per SM hold them all and each has a full ring (64
+  // rows of 129,280 logits with five alternatives: 15.2 us by 4, 16.4 by 8, 19.3 by
+  // 2; 40 rows 13.4 by 8, 14.4 by 4; 300 rows 40.5 by 1, 44.1 by 2)
   a.splits = 1;
-  while (a.splits < kLpCluster && 2LL * rows * a.splits <= 4LL * sms &&
+  while (a.splits < kLpCluster && 2LL * rows * a.splits <= 3LL * sms &&
          a.vocab > 4LL * kLpTurn * kLpWarps * a.splits)
     a.splits *= 2;
   cudaLaunchAttribute attr[2];

@@ -191,25 +191,24 @@ class KvCache:
 def _rows(t, rows, width: int, what: str):
     """Checks [rows x width] FP32 CUDA rows (rows None: any number) and returns
     (rows, floats between rows)."""
-    import torch
-
+    shape = t.shape
+    if len(shape) == 2 and t.is_cuda:
+        n, w = shape
+        between, apart = t.stride()
+        if (w == width and (n == rows or rows is None) and (apart == 1 or w == 1)
+                and (between >= w or n <= 1) and t.element_size() == 4 and t.is_floating_point()):
+            return n, between if n > 1 else w
     from . import OcrError
-    if t.dtype != torch.float32 or not t.is_cuda:
-        raise OcrError(4, f"invalid tensor shape: {what}: FP32 CUDA rows expected")
-    if t.dim() == 1:
-        t = t[None]
-    if t.dim() != 2 or t.shape[1] != width or (rows is not None and t.shape[0] != rows):
-        raise OcrError(4, f"invalid tensor shape: {what}: expected "
-                          f"{['rows' if rows is None else rows, width]}, got {list(t.shape)}")
-    if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
-        raise OcrError(4, f"invalid tensor shape: {what}: rows of adjacent floats expected")
-    return t.shape[0], t.stride(0) if t.shape[0] > 1 else width
+    raise OcrError(4, f"invalid tensor shape: {what}: FP32 CUDA rows "
+                      f"{['rows' if rows is None else rows, width]} of adjacent floats expected, got "
+                      f"{list(shape)} {t.dtype} on {t.device}")
 
 
 class QuantizedKvCache:
     """LayerCache for `batch` sequences held in `bits` (4 or 8) bits a dim plus
     a step and a least value per 32 dims of a head (uocr_kvq): ``KvCache``'s
-    calls, FP32 rows in and out.  Rows may lie apart (slices of wider rows)."""
+    calls, FP32 rows in and out.  Rows of keys and values may lie apart (slices
+    of wider rows)."""
 
     def __init__(self, ctx: GpuContext, batch: int, heads: int, head_dim: int, window: int,
                  max_prefix: int, bits: int = 4):
@@ -217,83 +216,88 @@ class QuantizedKvCache:
         self.batch, self.heads, self.head_dim, self.bits = batch, heads, head_dim, bits
         self.width = heads * head_dim
         h = ctypes.c_void_p()
-        _check(lib().uocr_kvq_create(ctx.handle, batch, heads, head_dim, window, max_prefix,
-                                     int(bits), ctypes.byref(h)))
+        self._lib = lib()
+        _check(self._lib.uocr_kvq_create(ctx.handle, batch, heads, head_dim, window, max_prefix,
+                                         int(bits), ctypes.byref(h)))
         self._h = h
 
     def storage_bytes(self) -> int:
-        return int(lib().uocr_kvq_storage_bytes(self._h))
+        return int(self._lib.uocr_kvq_storage_bytes(self._h))
+
+    def _whole(self, t, rows: int, width: int, what: str) -> int:
+        """Checks contiguous rows and returns their address."""
+        if _rows(t, rows, width, what)[1] != width:
+            from . import OcrError
+            raise OcrError(4, f"invalid tensor shape: {what}: contiguous rows expected")
+        return t.data_ptr()
 
     def prefill(self, seq: int, keys_t, values_t):
         """The rows of a prompt into the empty sequence seq."""
         tokens, ld_k = _rows(keys_t, None, self.width, "keys")
-        _, ld_v = _rows(values_t, tokens, self.width, "values")
-        _check(lib().uocr_kvq_prefill(self.ctx.handle, self._h, seq, _p(keys_t), ld_k, _p(values_t),
-                                      ld_v, tokens))
+        ld_v = _rows(values_t, tokens, self.width, "values")[1]
+        _check(self._lib.uocr_kvq_prefill(self.ctx.handle, self._h, seq, keys_t.data_ptr(), ld_k,
+                                          values_t.data_ptr(), ld_v, tokens))
 
     def push(self, k_t, v_t):
         """Row b of k and v into every sequence b."""
-        _, ld_k = _rows(k_t, self.batch, self.width, "k")
-        _, ld_v = _rows(v_t, self.batch, self.width, "v")
-        _check(lib().uocr_kvq_push(self.ctx.handle, self._h, _p(k_t), ld_k, _p(v_t), ld_v))
-
-    def _whole(self, t, rows: int, width: int, what: str):
-        from . import OcrError
-        _, ld = _rows(t, rows, width, what)
-        if ld != width:
-            raise OcrError(4, f"invalid tensor shape: {what}: contiguous rows expected")
-        return t
+        ld_k = _rows(k_t, self.batch, self.width, "k")[1]
+        ld_v = _rows(v_t, self.batch, self.width, "v")[1]
+        _check(self._lib.uocr_kvq_push(self.ctx.handle, self._h, k_t.data_ptr(), ld_k,
+                                       v_t.data_ptr(), ld_v))
 
     def rope(self, rope: Rope, q_t, k_t):
-        self._whole(q_t, self.batch, self.width, "q")
-        if k_t is not None:
-            self._whole(k_t, self.batch, self.width, "k")
-        _check(lib().uocr_kvq_rope(self.ctx.handle, self._h, rope._h, _p(q_t), _p(k_t)))
+        q = self._whole(q_t, self.batch, self.width, "q")
+        k = self._whole(k_t, self.batch, self.width, "k") if k_t is not None else None
+        _check(self._lib.uocr_kvq_rope(self.ctx.handle, self._h, rope._h, q, k))
 
     def rope_push_qkv(self, rope: Rope, qkv_t, q_out_t=None):
         """rope + push from fused projection rows [q | k | v]; returns the
         rotated q rows (uocr_kvq_rope_push_qkv)."""
-        import torch
-        self._whole(qkv_t, self.batch, 3 * self.width, "qkv")
-        q_out_t = q_out_t if q_out_t is not None else torch.empty(
-            (self.batch, self.width), device=qkv_t.device)
-        self._whole(q_out_t, self.batch, self.width, "q_out")
-        _check(lib().uocr_kvq_rope_push_qkv(self.ctx.handle, self._h, rope._h, _p(qkv_t),
-                                            _p(q_out_t)))
+        qkv = self._whole(qkv_t, self.batch, 3 * self.width, "qkv")
+        q_out_t = q_out_t if q_out_t is not None else qkv_t.new_empty((self.batch, self.width))
+        _check(self._lib.uocr_kvq_rope_push_qkv(
+            self.ctx.handle, self._h, rope._h, qkv,
+            self._whole(q_out_t, self.batch, self.width, "q_out")))
         return q_out_t
 
     def attention(self, q_t, out_t=None):
         """softmax(q K^T / sqrt(head_dim)) V of row b of q over sequence b."""
-        import torch
-        self._whole(q_t, self.batch, self.width, "q")
-        out_t = out_t if out_t is not None else torch.empty_like(q_t)
-        self._whole(out_t, self.batch, self.width, "out")
-        _check(lib().uocr_kvq_attention(self.ctx.handle, self._h, _p(q_t), _p(out_t)))
+        q = self._whole(q_t, self.batch, self.width, "q")
+        out_t = out_t if out_t is not None else q_t.new_empty((self.batch, self.width))
+        _check(self._lib.uocr_kvq_attention(self.ctx.handle, self._h, q,
+                                            self._whole(out_t, self.batch, self.width, "out")))
         return out_t
 
     def reset(self, seq: int):
         """Sequence seq empty again, to be prefilled anew."""
-        _check(lib().uocr_kvq_reset(self.ctx.handle, self._h, seq))
+        _check(self._lib.uocr_kvq_reset(self.ctx.handle, self._h, seq))
 
     def state(self, seq: int):
         """(tokens, position) of sequence seq (synchronous)."""
         t, p = ctypes.c_size_t(), ctypes.c_size_t()
-        _check(lib().uocr_kvq_state(self.ctx.handle, self._h, seq, ctypes.byref(t), ctypes.byref(p)))
+        _check(self._lib.uocr_kvq_state(self.ctx.handle, self._h, seq, ctypes.byref(t),
+                                        ctypes.byref(p)))
         return t.value, p.value
 
     def read(self, seq: int, first: int, count: int, keys_t=None, values_t=None):
         """What slots [first, first + count) of sequence seq stand for:
         token-major rows [count x width] of keys and of values."""
         import torch
-        dev = f"cuda:{self.ctx.device}"
-        keys_t, values_t = (t if t is not None else torch.empty((count, self.width), device=dev)
+        shape = (count, self.width)
+        keys_t, values_t = (t if t is not None else
+                            torch.empty(shape, dtype=torch.float32, device=self._device())
                             for t in (keys_t, values_t))
-        if count:
-            self._whole(keys_t, count, self.width, "keys")
-            self._whole(values_t, count, self.width, "values")
-        _check(lib().uocr_kvq_read(self.ctx.handle, self._h, seq, first, count, _p(keys_t),
-                                   _p(values_t)))
+        k = self._whole(keys_t, count, self.width, "keys")
+        v = self._whole(values_t, count, self.width, "values")
+        _check(self._lib.uocr_kvq_read(self.ctx.handle, self._h, seq, first, count, k, v))
         return keys_t, values_t
+
+    def _device(self):
+        import torch
+        device = getattr(self, "_torch_device", None)
+        if device is None:
+            device = self._torch_device = torch.device("cuda", self.ctx.device)
+        return device
 
     def export(self, seq: int):
         """``read`` of every token of sequence seq (synchronous)."""
@@ -301,7 +305,7 @@ class QuantizedKvCache:
 
     def free(self):
         if getattr(self, "_h", None):
-            lib().uocr_kvq_free(self._h)
+            self._lib.uocr_kvq_free(self._h)
             self._h = None
 
     def __del__(self):

@@ -332,26 +332,26 @@ def token_logprobs_device(ctx: GpuContext, logits_t, tokens_t=None, top_k: int =
     (uocr_token_logprobs).  -inf bans a token.  Asynchronous."""
     import torch
 
-    from . import OcrError
-    if logits_t.dim() != 2 or logits_t.dtype != torch.float32 or not logits_t.is_cuda:
-        raise OcrError(4, "invalid tensor shape: logits: FP32 CUDA rows [rows x vocab] expected")
-    rows, vocab = logits_t.shape
-    if (vocab > 1 and logits_t.stride(1) != 1) or (rows > 1 and logits_t.stride(0) < vocab):
-        raise OcrError(4, "invalid tensor shape: logits: rows of adjacent floats expected")
+    from .attention import _rows
+    rows, vocab = logits_t.shape if logits_t.dim() == 2 else (0, 0)
+    between = _rows(logits_t, rows, vocab, "logits")[1]
     if tokens_t is not None and (tokens_t.dtype != torch.int64 or not tokens_t.is_cuda
                                  or tokens_t.shape != (rows,) or not tokens_t.is_contiguous()):
+        from . import OcrError
         raise OcrError(4, "invalid tensor shape: tokens: contiguous int64 CUDA [rows] expected")
     if top_k < 0:
+        from . import OcrError
         raise OcrError(4, "invalid tensor shape: top_k must not be negative")
-    new = lambda *shape, **kw: torch.empty(shape, device=logits_t.device, **kw)  # noqa: E731
-    out = TokenLogprobs(new(rows) if tokens_t is not None else None, new(rows),
-                        new(rows, top_k, dtype=torch.int64), new(rows, top_k))
-    opt = lambda t: _p(t) if t is not None and t.numel() else None  # noqa: E731
-    _check(lib().uocr_token_logprobs(ctx.handle, _p(logits_t), rows, vocab,
-                                     logits_t.stride(0) if rows > 1 else vocab, opt(tokens_t),
-                                     top_k, opt(out.logprob), _p(out.entropy), opt(out.top_ids),
-                                     opt(out.top_logprobs)))
-    return out
+    new = logits_t.new_empty
+    logprob = new((rows,)) if tokens_t is not None else None
+    entropy = new((rows,))
+    ids, logprobs = new((rows, top_k), dtype=torch.int64), new((rows, top_k))
+    _check(lib().uocr_token_logprobs(
+        ctx.handle, logits_t.data_ptr(), rows, vocab, between,
+        tokens_t.data_ptr() if tokens_t is not None else None, top_k,
+        logprob.data_ptr() if logprob is not None else None, entropy.data_ptr(),
+        ids.data_ptr() if top_k else None, logprobs.data_ptr() if top_k else None))
+    return TokenLogprobs(logprob, entropy, ids, logprobs)
 
 
 def score_step(decoder: Decoder, state: DecodeState, tokens_t, next_t, mode: int = 0, top_k: int = 0,
