@@ -1965,7 +1965,8 @@ int uocr_kvq_reset(uocr_ctx* ctx, uocr_kvq* kv, size_t seq) {
   if (seq >= static_cast<size_t>(kv->batch))
     return fail(UOCR_ERR_SHAPE, "invalid tensor shape: cache sequence");
   DeviceGuard g(ctx->device);
-  CUDA_TRY(cudaMemsetAsync(kv->state + 2 * seq, 0, 2 * sizeof(int), ctx->stream));
+  launch_kvq_reset(kv->state, static_cast<int>(seq), ctx->stream);
+  if ((st = check_launch())) return st;
   kv->prefix[seq] = 0;
   return ok();
 }

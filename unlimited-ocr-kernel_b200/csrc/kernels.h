@@ -348,6 +348,8 @@ cudaError_t launch_attention_decode_tma(const AttnMaps& m, const AttnArgs& a, in
 void launch_kvq_prefill(unsigned char* data, const KvqLayout& L, int* state, int seq, const float* k,
                         long long ld_k, const float* v, long long ld_v, int tokens,
                         unsigned* status, cudaStream_t st);
+// {0, 0} as the state of sequence seq.
+void launch_kvq_reset(int* state, int seq, cudaStream_t st);
 // Row b into the next slot of every sequence b.
 void launch_kvq_push(unsigned char* data, const KvqLayout& L, int* state, int batch, int window,
                      const float* k, long long ld_k, const float* v, long long ld_v,

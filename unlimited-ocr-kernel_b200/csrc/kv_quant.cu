@@ -45,33 +45,64 @@ __device__ __forceinline__ float rcp_fast(float x) {  // 1 ulp; subnormals count
   return y;
 }
 
+// Largest and least of three and of two; NaN where one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// A group whose extremes hi and -lo are not both below 2^100 in magnitude, or are
+// NaN, is refused.
+__device__ __forceinline__ bool kvq_refused(float hi, float neg_lo) {
+  return !(fmaxf(hi, neg_lo) < 1.2676506e30f) || isnan(hi) || isnan(neg_lo);
+}
+
+constexpr float kKvqTinyStep = 1e-30f;  // steps below it (0 among them) go by double
+
 // Codes of four values as the bytes of a word: in float, rounded by adding
-// 1.5 2^23 (whose last place is 1), and again in double where a quotient is too
-// near a border between two codes, or the step too small, to decide.  The float
-// quotient is off by four roundings of 2^-24 at most, so by 6e-5 at 255.
-__device__ __forceinline__ uint32_t kvq_codes4(const float (&x)[4], float m, float s, float inv_s,
-                                               int levels) {
-  uint32_t c[4];
-  float worst = 0.0f;
-#pragma unroll
+// 1.5 2^23 (whose last place is 1).  *near is how far the quotients are from their
+// codes.  The float quotient is off by four roundings of 2^-24 at most, so by 6.1e-5
+// at 255 and 3.6e-6 at 15: from kvq_near on it is too near a border between two
+// codes to decide.
+constexpr float kvq_near(int bits) { return bits == 4 ? 0.499995f : 0.49993f; }
+__device__ __forceinline__ uint32_t kvq_codes4(const float (&x)[4], float m, float inv_s, float* near) {
+  const float2 nm = make_float2(-m, -m), is = make_float2(inv_s, inv_s);
+  const float2 magic = make_float2(12582912.0f, 12582912.0f), back = make_float2(-12582912.0f, -12582912.0f);
+  const float2 t0 = f2_mul(f2_add(make_float2(x[0], x[1]), nm), is);
+  const float2 t1 = f2_mul(f2_add(make_float2(x[2], x[3]), nm), is);
+  const float2 r0 = f2_add(t0, magic), r1 = f2_add(t1, magic);
+  const float2 o0 = f2_fma(f2_add(r0, back), make_float2(-1.0f, -1.0f), t0);
+  const float2 o1 = f2_fma(f2_add(r1, back), make_float2(-1.0f, -1.0f), t1);
+  *near = fmaxf(fmaxf(fabsf(o0.x), fabsf(o0.y)), fmaxf(fabsf(o1.x), fabsf(o1.y)));
+  return __byte_perm(__byte_perm(__float_as_uint(r0.x), __float_as_uint(r0.y), 0x0040),
+                     __byte_perm(__float_as_uint(r1.x), __float_as_uint(r1.y), 0x0040), 0x5410);
+}
+
+// The same by the definition, in double.
+__device__ __noinline__ uint32_t kvq_codes4_exactly(float x0, float x1, float x2, float x3, float m,
+                                                    float s, int levels) {
+  const float x[4] = {x0, x1, x2, x3};
+  uint32_t c = 0;
+#pragma unroll 1
   for (int i = 0; i < 4; ++i) {
-    const float t = __fmul_rn(__fsub_rn(x[i], m), inv_s);
-    const float r = __fadd_rn(t, 12582912.0f);
-    c[i] = __float_as_uint(r);
-    const float off = fabsf(__fsub_rn(t, __fsub_rn(r, 12582912.0f)));
-    worst = off < 0.4999f ? worst : 1.0f;  // (1 for NaN as well)
+    int v = 0;
+    if (s > 0.0f)
+      v = __double2int_rn(__ddiv_rn(__dsub_rn(static_cast<double>(x[i]), static_cast<double>(m)),
+                                    static_cast<double>(s)));
+    c |= static_cast<uint32_t>(min(max(v, 0), levels)) << (8 * i);
   }
-  if (worst != 0.0f || s < 1e-30f) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      int v = 0;
-      if (s > 0.0f)
-        v = __double2int_rn(__ddiv_rn(__dsub_rn(static_cast<double>(x[i]), static_cast<double>(m)),
-                                      static_cast<double>(s)));
-      c[i] = static_cast<uint32_t>(min(max(v, 0), levels));
-    }
-  }
-  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  return c;
 }
 
 // Four values of a row from dim d (a multiple of 4); zeros past the row's end.
@@ -90,17 +121,19 @@ __device__ __forceinline__ void kvq_load4(const float* row, int d, int dim, floa
   }
 }
 
-// Whether one of four values is not below 2^100 in magnitude.
-__device__ __forceinline__ bool kvq_refused(const float (&x)[4]) {
-  uint32_t u = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) u = max(u, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  return u >= 0x71800000u;
-}
-
 __device__ __forceinline__ unsigned char* kvq_tile(unsigned char* data, const KvqLayout& L, int seq,
                                                    int head, long long slot) {
   return data + ((static_cast<long long>(seq) * L.heads + head) * L.tiles + (slot >> 5)) * L.tile;
+}
+
+__global__ void kvq_reset_kernel(int* state, int seq) {
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  state[2 * seq] = state[2 * seq + 1] = 0;
+}
+
+void launch_kvq_reset(int* state, int seq, cudaStream_t st) {
+  launch_dependent(kvq_reset_kernel, dim3(1), dim3(1), 0, st, state, seq);
 }
 
 // ---- a prompt's rows ------------------------------------------------------------
@@ -110,12 +143,17 @@ __device__ __forceinline__ unsigned char* kvq_tile(unsigned char* data, const Kv
 // tokens are eight values over eight lanes: halving what a lane keeps at every
 // exchange takes 7 shuffles instead of 24 and leaves the extremes of token u in
 // the lanes u and u + 4 of the eight, which then find its parameters once.
+// VEC: rows that four floats at a time can be read from, so that a lane's four dims
+// are the row's or not as one.  (Five CTAs per SM, 48 registers: a prompt of 32,768
+// tokens takes 94 us with them, 8 bits, 107 with three and 104 with six.)
 template <int BITS, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 5)
     kvq_prefill_kernel(unsigned char* data, const KvqLayout L, int* state, int seq,
                        const float* __restrict__ k, long long ld_k, const float* __restrict__ v,
                        long long ld_v, int tokens, unsigned* status) {
   extern __shared__ __align__(16) unsigned char kvq_stage[];
+  pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
+  pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   constexpr int levels = (1 << BITS) - 1;
   const int h = blockIdx.x % L.heads, tile = blockIdx.x / L.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7;
@@ -125,6 +163,7 @@ __global__ void __launch_bounds__(256)
   }
   const int t0 = tile * 32 + warp * 4;  // this warp's tokens: t0 .. t0 + 3
   const int half = warp >> 2, j = warp & 3;
+  const bool h4 = l8 & 4, h2 = l8 & 2, h1 = l8 & 1;
   for (int q = 0; q < (L.groups + 3) / 4; ++q) {
     const int grp = q * 4 + (lane >> 3), d0 = grp * 32 + l8 * 4;
     const bool real = grp < L.groups;
@@ -133,64 +172,72 @@ __global__ void __launch_bounds__(256)
       const float* rows = (part ? v : k) + static_cast<long long>(h) * L.dim;
       const long long ld = part ? ld_v : ld_k;
       float x[4][4];
-      bool refused = false;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if (t0 + u < tokens) {
           kvq_load4<VEC>(rows + (t0 + u) * ld, d0, L.dim, x[u]);
         } else {
-          x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[u][i] = 0.0f;
         }
       }
       // the largest x and the largest -x of each token, over this lane's dims
       float a[4], b[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        refused |= kvq_refused(x[u]);
         a[u] = b[u] = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (d0 + i < L.dim) {
-            a[u] = fmaxf(a[u], x[u][i]);
-            b[u] = fmaxf(b[u], -x[u][i]);
+        if (VEC) {
+          if (d0 < L.dim) {
+            a[u] = max_nan(max3_nan(x[u][0], x[u][1], x[u][2]), x[u][3]);
+            b[u] = max_nan(-min3_nan(x[u][0], x[u][1], x[u][2]), -x[u][3]);
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (d0 + i < L.dim) {
+              a[u] = max_nan(a[u], x[u][i]);
+              b[u] = max_nan(b[u], -x[u][i]);
+            }
+        }
       }
-      const bool h4 = l8 & 4, h2 = l8 & 2, h1 = l8 & 1;
       float e[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        e[u] = fmaxf(h4 ? b[u] : a[u], __shfl_xor_sync(0xffffffffu, h4 ? a[u] : b[u], 4));
-      const float e0 = fmaxf(h2 ? e[2] : e[0], __shfl_xor_sync(0xffffffffu, h2 ? e[0] : e[2], 2));
-      const float e1 = fmaxf(h2 ? e[3] : e[1], __shfl_xor_sync(0xffffffffu, h2 ? e[1] : e[3], 2));
-      const float mine = fmaxf(h1 ? e1 : e0, __shfl_xor_sync(0xffffffffu, h1 ? e0 : e1, 1));
+        e[u] = max_nan(h4 ? b[u] : a[u], __shfl_xor_sync(0xffffffffu, h4 ? a[u] : b[u], 4));
+      const float e0 = max_nan(h2 ? e[2] : e[0], __shfl_xor_sync(0xffffffffu, h2 ? e[0] : e[2], 2));
+      const float e1 = max_nan(h2 ? e[3] : e[1], __shfl_xor_sync(0xffffffffu, h2 ? e[1] : e[3], 2));
+      const float mine = max_nan(h1 ? e1 : e0, __shfl_xor_sync(0xffffffffu, h1 ? e0 : e1, 1));
       const float other = __shfl_xor_sync(0xffffffffu, mine, 4);
+      const bool lost = real && kvq_refused(mine, other);  // of token l8 & 3: it reads as NaN
       float s, m;
       uint32_t word = kvq_params(-(h4 ? mine : other), h4 ? other : mine, 1.0 / levels, levels, &s, &m);
       const float inv_s = rcp_fast(s);
-      // a group that holds a refused value reads as NaN
-      unsigned lost = 0;
-      if (__any_sync(0xffffffffu, refused)) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if ((__ballot_sync(0xffffffffu, kvq_refused(x[u])) >> (lane & 24)) & 0xFFu) lost |= 1u << u;
-        if (lost) flag(status, DEV_KV_RANGE);
-        if ((lost >> (l8 & 3)) & 1) word = 0x7FC00000u;
-      }
+      if (lost) word = 0x7FC00000u;
       unsigned char* codes = kvq_stage + part * L.half;
       if (real && l8 < 4)
         *reinterpret_cast<uint32_t*>(codes + L.codes + kvq_param_byte(warp * 4 + l8, grp)) = word;
       uint32_t c[4];
+      const bool odd = real && (s < kKvqTinyStep || lost);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int from = (lane & 24) + u;
-        c[u] = kvq_codes4(x[u], __shfl_sync(0xffffffffu, m, from), __shfl_sync(0xffffffffu, s, from),
-                          __shfl_sync(0xffffffffu, inv_s, from), levels);
-        if ((lost >> u) & 1) c[u] = 0;
-        if (d0 + 3 >= L.dim) {
+        const float mu = __shfl_sync(0xffffffffu, m, from);
+        float near;
+        c[u] = kvq_codes4(x[u], mu, __shfl_sync(0xffffffffu, inv_s, from), &near);
+        if (__any_sync(0xffffffffu, near >= kvq_near(BITS) || (odd && (l8 & 3) == u))) {
+          const float su = __shfl_sync(0xffffffffu, s, from);
+          if (near >= kvq_near(BITS) || su < kKvqTinyStep)
+            c[u] = kvq_codes4_exactly(x[u][0], x[u][1], x[u][2], x[u][3], mu, su, levels);
+          if (__shfl_sync(0xffffffffu, lost, from)) c[u] = 0;
+        }
+      }
+      if (lost) flag(status, DEV_KV_RANGE);
+      if (d0 + 3 >= L.dim) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (d0 + i >= L.dim) c[u] &= ~(0xFFu << (8 * i));
-        }
       }
       if (part == 0) {
 #pragma unroll
@@ -235,15 +282,18 @@ void launch_kvq_prefill(unsigned char* data, const KvqLayout& L, int* state, int
   auto kernel = L.bits == 4 ? vec ? kvq_prefill_kernel<4, true> : kvq_prefill_kernel<4, false>
                 : vec       ? kvq_prefill_kernel<8, true>
                             : kvq_prefill_kernel<8, false>;
-  kernel<<<blocks, 256, L.tile, st>>>(data, L, state, seq, k, ld_k, v, ld_v, tokens, status);
+  launch_dependent(kernel, dim3(blocks), dim3(256), static_cast<size_t>(L.tile), st, data, L, state, seq, k,
+                   ld_k, v, ld_v, tokens, status);
 }
 
 // ---- one token of every sequence ----------------------------------------------------
 // One CTA per sequence, one warp per head and key or value; lanes as above, the
 // token's bytes straight into the tile.  ROPE: the rows are the fused projections
 // [q | k | v]; q is rotated into q_out and k rotated before it is quantised.
+constexpr int kKvqPushWarps = 20;
+
 template <int BITS, bool ROPE>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(kKvqPushWarps * 32)
     kvq_push_kernel(unsigned char* data, const KvqLayout L, int* state, int window,
                     const float* __restrict__ k, long long ld_k, const float* __restrict__ v,
                     long long ld_v, float* q_out, const float2* __restrict__ table, int max_pos,
@@ -284,29 +334,30 @@ __global__ void __launch_bounds__(1024)
     for (int q = 0; q < (L.groups + 3) / 4; ++q) {
       const int grp = q * 4 + (lane >> 3), d0 = grp * 32 + l8 * 4;
       const bool real = grp < L.groups;
-      float x[4], hi = -INFINITY, lo = INFINITY;
+      float x[4], hi = -INFINITY, neg_lo = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = d0 + i;
         x[i] = 0.0f;
         if (d < L.dim) {
           x[i] = ROPE && !value ? rotated(row, d) : row[d];
-          hi = fmaxf(hi, x[i]);
-          lo = fminf(lo, x[i]);
+          hi = max_nan(hi, x[i]);
+          neg_lo = max_nan(neg_lo, -x[i]);
         }
       }
 #pragma unroll
       for (int o = 1; o <= 4; o <<= 1) {
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        neg_lo = max_nan(neg_lo, __shfl_xor_sync(0xffffffffu, neg_lo, o));
       }
-      float s, m;
-      uint32_t word = kvq_params(lo, hi, 1.0 / levels, levels, &s, &m);
-      uint32_t c = kvq_codes4(x, m, s, rcp_fast(s), levels);
+      float s, m, near;
+      uint32_t word = kvq_params(-neg_lo, hi, 1.0 / levels, levels, &s, &m);
+      uint32_t c = kvq_codes4(x, m, rcp_fast(s), &near);
+      if (near >= kvq_near(BITS) || s < kKvqTinyStep) c = kvq_codes4_exactly(x[0], x[1], x[2], x[3], m, s, levels);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (d0 + i >= L.dim) c &= ~(0xFFu << (8 * i));
-      if ((__ballot_sync(0xffffffffu, kvq_refused(x)) >> (lane & 24)) & 0xFFu) {  // reads as NaN
+      if (real && kvq_refused(hi, neg_lo)) {  // reads as NaN
         word = 0x7FC00000u;
         c = 0;
         flag(status, DEV_KV_RANGE);
@@ -332,7 +383,9 @@ __global__ void __launch_bounds__(1024)
   if (threadIdx.x == 0) state[2 * b + 1] = gen + 1;
 }
 
-static int push_threads(const KvqLayout& L) { return 32 * (2 * L.heads < 32 ? 2 * L.heads : 32); }
+static int push_threads(const KvqLayout& L) {
+  return 32 * (2 * L.heads < kKvqPushWarps ? 2 * L.heads : kKvqPushWarps);
+}
 
 void launch_kvq_push(unsigned char* data, const KvqLayout& L, int* state, int batch, int window,
                      const float* k, long long ld_k, const float* v, long long ld_v,
@@ -366,6 +419,8 @@ __global__ void __launch_bounds__(256)
                     const int* __restrict__ state, int window, int seq, long long first,
                     long long count, float* k, float* v, unsigned* status) {
   extern __shared__ __align__(16) unsigned char kvq_stage[];
+  pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
+  pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   const int h = blockIdx.x % L.heads;
   const long long tile = (first >> 5) + blockIdx.x / L.heads;
   const uint4* in = reinterpret_cast<const uint4*>(
@@ -422,7 +477,8 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
   auto kernel = L.bits == 4 ? vec ? kvq_read_kernel<4, true> : kvq_read_kernel<4, false>
                 : vec       ? kvq_read_kernel<8, true>
                             : kvq_read_kernel<8, false>;
-  kernel<<<blocks, 256, L.tile, st>>>(data, L, state, window, seq, first, count, k, v, status);
+  launch_dependent(kernel, dim3(blocks), dim3(256), static_cast<size_t>(L.tile), st, data, L, state, window,
+                   seq, first, count, k, v, status);
 }
 
 // ---- attention -------------------------------------------------------------------

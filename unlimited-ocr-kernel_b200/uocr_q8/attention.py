@@ -282,22 +282,21 @@ class QuantizedKvCache:
     def read(self, seq: int, first: int, count: int, keys_t=None, values_t=None):
         """What slots [first, first + count) of sequence seq stand for:
         token-major rows [count x width] of keys and of values."""
-        import torch
-        shape = (count, self.width)
-        keys_t, values_t = (t if t is not None else
-                            torch.empty(shape, dtype=torch.float32, device=self._device())
-                            for t in (keys_t, values_t))
+        if keys_t is None:
+            keys_t = self._new(count)
+        if values_t is None:
+            values_t = self._new(count)
         k = self._whole(keys_t, count, self.width, "keys")
         v = self._whole(values_t, count, self.width, "values")
         _check(self._lib.uocr_kvq_read(self.ctx.handle, self._h, seq, first, count, k, v))
         return keys_t, values_t
 
-    def _device(self):
-        import torch
-        device = getattr(self, "_torch_device", None)
-        if device is None:
-            device = self._torch_device = torch.device("cuda", self.ctx.device)
-        return device
+    def _new(self, rows: int):
+        like = getattr(self, "_like", None)
+        if like is None:
+            import torch
+            like = self._like = torch.empty(0, dtype=torch.float32, device=f"cuda:{self.ctx.device}")
+        return like.new_empty((rows, self.width))
 
     def export(self, seq: int):
         """``read`` of every token of sequence seq (synchronous)."""
