@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(256, 5)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (BITS == 4) c[u] |= __shfl_xor_sync(0xffffffffu, c[u], 4) << 4;
+          c[u] ^= kvq_flip(BITS);
           if (real && (BITS == 8 || !h4))
             *reinterpret_cast<uint32_t*>(codes + kvq_key_byte(warp * 4 + u, d0, BITS)) = c[u];
         }
@@ -255,6 +256,7 @@ __global__ void __launch_bounds__(256, 5)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (BITS == 4) w[i] |= __shfl_xor_sync(0xffffffffu, w[i], 2) << 4;
+          w[i] ^= kvq_flip(BITS);
           if (real && (BITS == 8 || !h2))
             *reinterpret_cast<uint32_t*>(codes + kvq_value_byte(half * 16 + j * 4, d0 + i, BITS)) = w[i];
         }
@@ -365,6 +367,7 @@ __global__ void __launch_bounds__(kKvqPushWarps * 32)
       if (real && l8 == 0) *reinterpret_cast<uint32_t*>(codes + L.codes + kvq_param_byte(t, grp)) = word;
       const uint32_t up = __shfl_xor_sync(0xffffffffu, c, value ? 2 : 4);
       if (BITS == 4) c |= up << 4;
+      c ^= kvq_flip(BITS);
       if (!real || (BITS == 4 && (l8 & (value ? 2 : 4)))) continue;
       if (!value) {
         *reinterpret_cast<uint32_t*>(codes + kvq_key_byte(t, d0, BITS)) = c;
@@ -444,6 +447,7 @@ __global__ void __launch_bounds__(256)
       for (int u = 0; u < 4; ++u) {
         c[u] = *reinterpret_cast<const uint32_t*>(
             codes + (part ? kvq_value_byte(warp * 4, d0 + u, BITS) : kvq_key_byte(warp * 4 + u, d0, BITS)));
+        c[u] ^= kvq_flip(BITS);
         if (BITS == 4) c[u] = (l8 & (part ? 2 : 4) ? c[u] >> 4 : c[u]) & 0x0F0F0F0Fu;
       }
 #pragma unroll
@@ -483,31 +487,34 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 
 // ---- attention -------------------------------------------------------------------
 // One query per (head, sequence) over the tiles of its cache.  The codes go to
-// the matrix unit as they are (u8, m16n8k32), the query and the softmax weights
-// as fixed-point numbers cut into bytes, one byte per column of the 8-wide
-// operand, so that every product is exact and nothing is dequantised:
+// the matrix unit nearly as they lie (s8, m16n8k32: c - C with C the middle of the
+// codes, 16 (c - 8) for 4 bits), the query and the softmax weights as fixed-point
+// numbers cut into bytes, one byte per column of the 8-wide operand, so that every
+// product is exact and nothing is dequantised.  With z = m + C s:
 //
 //   scores:  rows = 16 tokens, k = the 32 dims of a group, columns = the four
 //            signed bytes of q 2^a (|q 2^a| < 2^30, a by the group's largest |q|);
-//            q . c = sum_b 256^b D_b, then s (q . c) + m sum(q) per group;
+//            q . (c - C) = sum_b 256^b D_b, then s (q . (c - C)) + z sum(q);
 //   values:  rows = 16 dims, k = the tile's 32 tokens, columns = the four bytes
 //            of p_t s_t 2^a (< 2^31, a by the largest s so far);
-//            o += 2^-a sum_b 256^b D_b, and p_t m_t is summed apart.
+//            o += 2^-a sum_b 256^b D_b, and p_t z_t is summed apart.
 //
+// Around the middle the sums stay near the size of what they stand for (from 0 up
+// they cancel against the least values, which cost a factor of two in accuracy).
 // Two neighbouring groups share an accumulator: a group's operand has its bytes
 // in its four columns and zeros in the other group's four.  Fixed point loses
-// less than a float does: 2^-31 of the group's largest |q|, 2^-32 of the
-// largest step, against a float's 2^-24 of each term.
+// less than a float does: 2^-31 of the group's largest |q|, 2^-30 of the largest
+// weight's size, against a float's 2^-24 of each term.
 //
 // A tile is one bulk copy.  Every warp has a ring of its own, takes a run of
 // neighbouring tiles, and keeps its own maximum, sum and weighted values, so the
 // loop has no barrier but the ring's.  The warps' parts are joined in shared
-// memory, the CTAs' of one head through distributed shared memory: one launch,
-// no workspace.
+// memory, the CTAs' of a cluster through distributed shared memory, the clusters'
+// of a head (where the heads are few) by the one that ends last.
 constexpr float kLog2e = 1.44269504f;
-// Weights stay below e^4 < 2^6 of the running maximum (see the loop).
-constexpr float kKvqSlack = 4.0f;
-constexpr int kKvqSlackBits = 6;
+// Scores may pass the running maximum by this much: weights stay below 2^2.
+constexpr float kKvqSlack = 1.38f;
+constexpr int kKvqSlackBits = 2;
 constexpr int kKvqSlots = 2;  // ring slots per warp
 constexpr int kKvqCluster = 8;  // most CTAs of a cluster (portable)
 
@@ -537,23 +544,27 @@ struct KvqShared {
   int turn;
 };
 
-// u8 rows times signed (SIGNED) or unsigned columns, 32-bit sums.
+// s8 rows times signed (SIGNED) or unsigned columns, 32-bit sums.
 template <bool SIGNED>
-__device__ __forceinline__ void mma_u8_m16n8k32(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+__device__ __forceinline__ void mma_s8_m16n8k32(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                                 uint32_t a3, uint32_t b0, uint32_t b1) {
   if (SIGNED)
     asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
         "{%8, %9}, {%0, %1, %2, %3};"
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
     asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
         "{%8, %9}, {%0, %1, %2, %3};"
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+
+// 16 times the signed nibbles of a word, as signed bytes.
+__device__ __forceinline__ uint32_t nibbles_low(uint32_t w) { return (w << 4) & 0xF0F0F0F0u; }
+__device__ __forceinline__ uint32_t nibbles_high(uint32_t w) { return w & 0xF0F0F0F0u; }
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; exact 1 at 0
   float y;
@@ -595,6 +606,8 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
   constexpr int N = Shared::N, W = Shared::W;
   constexpr int kTileBytes = kvq_tile_bytes(G, BITS);
   constexpr int kCodes = G * 512 * (BITS / 4);
+  constexpr float kMiddle = 1 << (BITS - 1);
+  constexpr int kShift = BITS == 4 ? 4 : 0;  // the operand is 2^kShift (c - kMiddle)
   extern __shared__ __align__(128) unsigned char kvq_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(kvq_raw);
   // a head: `parts` clusters of `splits` CTAs
@@ -673,16 +686,16 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
     const int ea = __shfl_sync(0xffffffffu, e, acc_group * 16);
     const float sa = __shfl_sync(0xffffffffu, sum, acc_group * 16);
     const bool real = 2 * p + acc_group < G;
-    qscale[p] = real ? __uint_as_float(static_cast<uint32_t>(min(ea, 254) - 29 + (j & 1) * 16) << 23) : 0.0f;
+    qscale[p] = real ? __uint_as_float(static_cast<uint32_t>(min(ea, 254) - 29 - kShift + (j & 1) * 16) << 23) : 0.0f;
     qsum[p] = real && !(j & 1) ? sa : 0.0f;
   }
 
-  float m = -INFINITY, l = 0.0f, least[G], o[P][2][2];
+  float m = -INFINITY, l = 0.0f, middle[G], o[P][2][2];
   uint32_t bound[G];    // largest step so far per group, as bf16 bits
   float wup[G], wdown[P];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
-    least[i] = 0.0f;
+    middle[i] = 0.0f;
     bound[i] = 0;
     wup[i] = 0.0f;
   }
@@ -721,15 +734,14 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
         uint4 lo, hi;
         if (BITS == 4) {
           const uint4 w = *reinterpret_cast<const uint4*>(kt + grp * 512 + lane * 16);
-          lo = make_uint4(w.x & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu, w.z & 0x0F0F0F0Fu, w.w & 0x0F0F0F0Fu);
-          hi = make_uint4((w.x >> 4) & 0x0F0F0F0Fu, (w.y >> 4) & 0x0F0F0F0Fu,
-                          (w.z >> 4) & 0x0F0F0F0Fu, (w.w >> 4) & 0x0F0F0F0Fu);
+          lo = make_uint4(nibbles_low(w.x), nibbles_low(w.y), nibbles_low(w.z), nibbles_low(w.w));
+          hi = make_uint4(nibbles_high(w.x), nibbles_high(w.y), nibbles_high(w.z), nibbles_high(w.w));
         } else {
           lo = *reinterpret_cast<const uint4*>(kt + grp * 1024 + lane * 16);
           hi = *reinterpret_cast<const uint4*>(kt + grp * 1024 + 512 + lane * 16);
         }
-        mma_u8_m16n8k32<true>(d[0][grp >> 1], lo.x, lo.y, hi.x, hi.y, qb[grp][0], qb[grp][1]);
-        mma_u8_m16n8k32<true>(d[1][grp >> 1], lo.z, lo.w, hi.z, hi.w, qb[grp][0], qb[grp][1]);
+        mma_s8_m16n8k32<true>(d[0][grp >> 1], lo.x, lo.y, hi.x, hi.y, qb[grp][0], qb[grp][1]);
+        mma_s8_m16n8k32<true>(d[1][grp >> 1], lo.z, lo.w, hi.z, hi.w, qb[grp][0], qb[grp][1]);
       }
       // x[i]: this lane's part of the score of token g + 8 i
       float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -742,7 +754,8 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
         for (int i = 0; i < 4; ++i) {
           const int (&dd)[4] = d[i >> 1][p];
           const float dot = static_cast<float>(dd[2 * (i & 1)] + (dd[2 * (i & 1) + 1] << 8)) * qscale[p];
-          x[i] = fmaf(bf16_low(par[i]), dot, fmaf(bf16_high(par[i]), qsum[p], x[i]));
+          const float step = bf16_low(par[i]);
+          x[i] = fmaf(step, dot, fmaf(fmaf(kMiddle, step, bf16_high(par[i])), qsum[p], x[i]));
         }
       }
       // the four lanes of a row add up and lane j keeps token t = g + 8 j
@@ -778,7 +791,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
         m = top;
         l *= keep;
 #pragma unroll
-        for (int i = 0; i < G; ++i) least[i] *= keep;
+        for (int i = 0; i < G; ++i) middle[i] *= keep;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
           o[p][0][0] *= keep;
@@ -800,7 +813,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const uint32_t bd = acc_group && 2 * p + 1 < G ? bound[min(2 * p + 1, G - 1)] : bound[2 * p];
-        wdown[p] = __uint_as_float((max(bd >> 7, 40u) - 30u + kKvqSlackBits + (j & 1) * 16u) << 23);
+        wdown[p] = __uint_as_float((max(bd >> 7, 40u) - 30u - kShift + kKvqSlackBits + (j & 1) * 16u) << 23);
       }
     }
     // ---- the weights' bytes
@@ -810,8 +823,9 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
       l += pr;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        least[i] = fmaf(pr, bf16_high(par[u][i]), least[i]);
-        sh.weights[warp][u][i][t] = __float2uint_rn(pr * (bf16_low(par[u][i]) * wup[i]));
+        const float step = bf16_low(par[u][i]);
+        middle[i] = fmaf(pr, fmaf(kMiddle, step, bf16_high(par[u][i])), middle[i]);
+        sh.weights[warp][u][i][t] = __float2uint_rn(pr * (step * wup[i]));
       }
     }
     __syncwarp();
@@ -834,19 +848,19 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
           const uint32_t c0 = col_group == c ? b0 : 0, c1 = col_group == c ? b1 : 0;
           if (BITS == 4) {
             const uint4 w = *reinterpret_cast<const uint4*>(vt + grp * 512 + lane * 16);
-            mma_u8_m16n8k32<false>(d[0], w.x & 0x0F0F0F0Fu, (w.x >> 4) & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu,
-                                   (w.y >> 4) & 0x0F0F0F0Fu, c0, c1);
-            mma_u8_m16n8k32<false>(d[1], w.z & 0x0F0F0F0Fu, (w.z >> 4) & 0x0F0F0F0Fu, w.w & 0x0F0F0F0Fu,
-                                   (w.w >> 4) & 0x0F0F0F0Fu, c0, c1);
+            mma_s8_m16n8k32<false>(d[0], nibbles_low(w.x), nibbles_high(w.x), nibbles_low(w.y),
+                                   nibbles_high(w.y), c0, c1);
+            mma_s8_m16n8k32<false>(d[1], nibbles_low(w.z), nibbles_high(w.z), nibbles_low(w.w),
+                                   nibbles_high(w.w), c0, c1);
           } else {
             const uint4 v0 = *reinterpret_cast<const uint4*>(vt + grp * 1024 + lane * 16);
             const uint4 v1 = *reinterpret_cast<const uint4*>(vt + grp * 1024 + 512 + lane * 16);
-            mma_u8_m16n8k32<false>(d[0], v0.x, v0.y, v0.z, v0.w, c0, c1);
-            mma_u8_m16n8k32<false>(d[1], v1.x, v1.y, v1.z, v1.w, c0, c1);
+            mma_s8_m16n8k32<false>(d[0], v0.x, v0.y, v0.z, v0.w, c0, c1);
+            mma_s8_m16n8k32<false>(d[1], v1.x, v1.y, v1.z, v1.w, c0, c1);
           }
         }
       }
-      // (sums of N tiles: at most 2 * 32 * 255 * 255 * 257 < 2^31)
+      // (sums of N tiles: at most 2 * 32 * 128 * 255 * 257 < 2^31)
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -869,7 +883,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
   // ---- the warps' parts
   l = warp_sum(l);
 #pragma unroll
-  for (int i = 0; i < G; ++i) least[i] = warp_sum(least[i]);
+  for (int i = 0; i < G; ++i) middle[i] = warp_sum(middle[i]);
 #pragma unroll
   for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -877,7 +891,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
 #pragma unroll
       for (int up = 0; up < 2; ++up) {
         const float v = o[p][mb][up] + __shfl_xor_sync(0xffffffffu, o[p][mb][up], 1);
-        const float add = acc_group && 2 * p + 1 < G ? least[min(2 * p + 1, G - 1)] : least[2 * p];
+        const float add = acc_group && 2 * p + 1 < G ? middle[min(2 * p + 1, G - 1)] : middle[2 * p];
         if (!(j & 1) && 2 * p + acc_group < G)
           sh.o[warp][(2 * p + acc_group) * 32 + mb * 16 + up * 8 + g] = v + add;
       }

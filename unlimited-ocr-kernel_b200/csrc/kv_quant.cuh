@@ -2,7 +2,8 @@
 //
 // A group is 32 consecutive dims of one head of one token's key (or value);
 // it holds a code per dim, a step s and a least value m (both bf16), and
-// stands for m + s * code.  The cache of one head of one sequence is a
+// stands for m + s * code.  A stored code is the code less the middle one (8 of
+// 16, 128 of 256) in two's complement: its highest bit flipped.  The cache of one head of one sequence is a
 // sequence of 32-token tiles, each one contiguous block
 //
 //   [key codes][key parameters][value codes][value parameters]
@@ -55,6 +56,9 @@ UOCR_HD KvqLayout kvq_layout(int heads, int dim, int bits, long long slots) {
   L.tiles = (slots + kKvqTile - 1) / kKvqTile;
   return L;
 }
+
+// What turns codes, byte by byte or nibble by nibble, into stored codes and back.
+UOCR_HD constexpr unsigned kvq_flip(int bits) { return bits == 4 ? 0x88888888u : 0x80808080u; }
 
 // Lane (and parameter word) of token t of a tile.
 UOCR_HD int kvq_lane(int t) { return (t & 7) * 4 + (t >> 3); }
