@@ -87,7 +87,7 @@ struct LpShared {
   uint64_t full[kLpWarps][kLpStages];
   float m[kLpWarps], s[kLpWarps], w[kLpWarps], n[kLpWarps];
   float part[4];                             // the CTA's {M, S, W, n}
-  uint32_t bound[kLpWarps];
+  uint32_t bound[2 * kLogprobMaxTop + kLpWarps];
   int count;                                 // candidates that have joined
   int over;                                  // more than the list holds
 };
@@ -187,24 +187,31 @@ struct LpRow {
   }
 };
 
-// The r-th best of every warp's 32 orders, r = ceil(k / warps): k threads reach
-// the least of them, and so do k elements.  A barrier before and after.
+// Raises the floor to the k-th best of the warps' best lanes: of the r best of each
+// warp's 32 orders, r = ceil(2 k / warps), which k elements reach.  A barrier
+// before and after.
 __device__ __noinline__ void lp_bound(LpShared& sh, uint32_t order, int k) {
-  uint32_t nth = 0;
+  const int r = (2 * k + kLpWarps - 1) / kLpWarps, n = r * kLpWarps;
 #pragma unroll 1
-  for (int r = 0; r < (k + kLpWarps - 1) / kLpWarps; ++r) {
-    nth = __reduce_max_sync(0xffffffffu, order);
-    const unsigned who = __ballot_sync(0xffffffffu, order == nth);
-    if ((threadIdx.x & 31) == __ffs(who) - 1) order = 0;
+  for (int i = 0; i < r; ++i) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, order);
+    const unsigned who = __ballot_sync(0xffffffffu, order == top);
+    if ((threadIdx.x & 31) == __ffs(who) - 1) {
+      order = 0;
+      sh.bound[(threadIdx.x >> 5) * r + i] = top;
+    }
   }
-  if ((threadIdx.x & 31) == 0) sh.bound[threadIdx.x >> 5] = nth;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    uint32_t low = sh.bound[0];
-#pragma unroll
-    for (int i = 1; i < kLpWarps; ++i) low = min(low, sh.bound[i]);
-    const LpKey floor = static_cast<LpKey>(low) << 32;
-    if (floor > sh.floor) sh.floor = floor;
+  if (threadIdx.x < n) {
+    const uint32_t mine = sh.bound[threadIdx.x];
+    int above = 0, reach = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      above += sh.bound[i] > mine;
+      reach += sh.bound[i] >= mine;
+    }
+    const LpKey floor = static_cast<LpKey>(mine) << 32;  // (equal ones write the same)
+    if (above < k && reach >= k && floor > sh.floor) sh.floor = floor;
   }
   __syncthreads();
 }
