@@ -188,16 +188,25 @@ class KvCache:
             pass
 
 
+_FP32 = None  # torch.float32, once torch has been imported
+
+
 def _rows(t, rows, width: int, what: str):
     """Checks [rows x width] FP32 CUDA rows (rows None: any number) and returns
     (rows, floats between rows)."""
+    global _FP32
+    if _FP32 is None:
+        import torch
+        _FP32 = torch.float32
     shape = t.shape
-    if len(shape) == 2 and t.is_cuda:
+    if len(shape) == 2 and t.dtype is _FP32 and t.is_cuda:
         n, w = shape
-        between, apart = t.stride()
-        if (w == width and (n == rows or rows is None) and (apart == 1 or w == 1)
-                and (between >= w or n <= 1) and t.element_size() == 4 and t.is_floating_point()):
-            return n, between if n > 1 else w
+        if w == width and (n == rows or rows is None):
+            between, apart = t.stride()
+            if apart == 1 and between == w or w == 1 and n <= 1:
+                return n, w
+            if (apart == 1 or w == 1) and (between >= w or n <= 1):
+                return n, between if n > 1 else w
     from . import OcrError
     raise OcrError(4, f"invalid tensor shape: {what}: FP32 CUDA rows "
                       f"{['rows' if rows is None else rows, width]} of adjacent floats expected, got "
@@ -254,18 +263,22 @@ class QuantizedKvCache:
         """rope + push from fused projection rows [q | k | v]; returns the
         rotated q rows (uocr_kvq_rope_push_qkv)."""
         qkv = self._whole(qkv_t, self.batch, 3 * self.width, "qkv")
-        q_out_t = q_out_t if q_out_t is not None else qkv_t.new_empty((self.batch, self.width))
-        _check(self._lib.uocr_kvq_rope_push_qkv(
-            self.ctx.handle, self._h, rope._h, qkv,
-            self._whole(q_out_t, self.batch, self.width, "q_out")))
+        if q_out_t is None:
+            q_out_t = qkv_t.new_empty((self.batch, self.width))
+        else:
+            self._whole(q_out_t, self.batch, self.width, "q_out")
+        _check(self._lib.uocr_kvq_rope_push_qkv(self.ctx.handle, self._h, rope._h, qkv,
+                                                q_out_t.data_ptr()))
         return q_out_t
 
     def attention(self, q_t, out_t=None):
         """softmax(q K^T / sqrt(head_dim)) V of row b of q over sequence b."""
         q = self._whole(q_t, self.batch, self.width, "q")
-        out_t = out_t if out_t is not None else q_t.new_empty((self.batch, self.width))
-        _check(self._lib.uocr_kvq_attention(self.ctx.handle, self._h, q,
-                                            self._whole(out_t, self.batch, self.width, "out")))
+        if out_t is None:
+            out_t = q_t.new_empty((self.batch, self.width))
+        else:
+            self._whole(out_t, self.batch, self.width, "out")
+        _check(self._lib.uocr_kvq_attention(self.ctx.handle, self._h, q, out_t.data_ptr()))
         return out_t
 
     def reset(self, seq: int):
@@ -284,11 +297,14 @@ class QuantizedKvCache:
         token-major rows [count x width] of keys and of values."""
         if keys_t is None:
             keys_t = self._new(count)
+        else:
+            self._whole(keys_t, count, self.width, "keys")
         if values_t is None:
             values_t = self._new(count)
-        k = self._whole(keys_t, count, self.width, "keys")
-        v = self._whole(values_t, count, self.width, "values")
-        _check(self._lib.uocr_kvq_read(self.ctx.handle, self._h, seq, first, count, k, v))
+        else:
+            self._whole(values_t, count, self.width, "values")
+        _check(self._lib.uocr_kvq_read(self.ctx.handle, self._h, seq, first, count,
+                                       keys_t.data_ptr(), values_t.data_ptr()))
         return keys_t, values_t
 
     def _new(self, rows: int):

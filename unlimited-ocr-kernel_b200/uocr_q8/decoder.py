@@ -29,7 +29,7 @@ from typing import List, NamedTuple, Optional
 import numpy as np
 
 from . import (GpuContext, Int8Matrix, MoeLayer, QuantizationMode, _check, _tptr, lib)
-from .attention import (KvCache, QuantizedKvCache, Rope, add_rms_norm_device,
+from .attention import (KvCache, QuantizedKvCache, Rope, _rows, add_rms_norm_device,
                         attention_prefill_device, rms_norm_device)
 
 
@@ -315,6 +315,9 @@ def logits_checksum_device(ctx: GpuContext, logits_t, acc_t):
     _check(lib().uocr_bits_checksum(ctx.handle, _p(logits_t), logits_t.numel(), _p(acc_t)))
 
 
+_INT64 = None  # torch.int64, once torch has been imported
+
+
 class TokenLogprobs(NamedTuple):
     """What rows of logits say: ``logprob`` [rows] of the given tokens (None
     without tokens), ``entropy`` [rows], ``top_ids`` (int64) and
@@ -330,12 +333,13 @@ def token_logprobs_device(ctx: GpuContext, logits_t, tokens_t=None, top_k: int =
     under the rows of logits_t [rows x vocab] (FP32, rows may lie apart), the
     rows' entropies and top_k most probable tokens, equal ones by the lower id
     (uocr_token_logprobs).  -inf bans a token.  Asynchronous."""
-    import torch
-
-    from .attention import _rows
+    global _INT64
+    if _INT64 is None:
+        import torch
+        _INT64 = torch.int64
     rows, vocab = logits_t.shape if logits_t.dim() == 2 else (0, 0)
     between = _rows(logits_t, rows, vocab, "logits")[1]
-    if tokens_t is not None and (tokens_t.dtype != torch.int64 or not tokens_t.is_cuda
+    if tokens_t is not None and (tokens_t.dtype is not _INT64 or not tokens_t.is_cuda
                                  or tokens_t.shape != (rows,) or not tokens_t.is_contiguous()):
         from . import OcrError
         raise OcrError(4, "invalid tensor shape: tokens: contiguous int64 CUDA [rows] expected")
@@ -345,7 +349,7 @@ def token_logprobs_device(ctx: GpuContext, logits_t, tokens_t=None, top_k: int =
     new = logits_t.new_empty
     logprob = new((rows,)) if tokens_t is not None else None
     entropy = new((rows,))
-    ids, logprobs = new((rows, top_k), dtype=torch.int64), new((rows, top_k))
+    ids, logprobs = new((rows, top_k), dtype=_INT64), new((rows, top_k))
     _check(lib().uocr_token_logprobs(
         ctx.handle, logits_t.data_ptr(), rows, vocab, between,
         tokens_t.data_ptr() if tokens_t is not None else None, top_k,
