@@ -560,3 +560,81 @@ def test_two_contexts_on_two_streams():
     for c, kv, *_ in made:
         kv.free()
         c.close()
+
+
+def test_first_calls_of_a_process_in_a_graph():
+    """Nothing has to run before a capture but the calls that make the cache: the
+    first push, attention and log probabilities of a process are captured."""
+    import subprocess
+    import sys
+    from conftest import PKG
+    code = f"""
+import sys
+sys.path.insert(0, {PKG!r})
+import torch, uocr_q8
+from uocr_q8.attention import QuantizedKvCache
+from uocr_q8.decoder import token_logprobs_device
+ctx = uocr_q8.GpuContext(0)
+side = torch.cuda.Stream()
+ctx.set_stream(side)
+kv = QuantizedKvCache(ctx, 2, 2, 64, 4, 50, 4)
+x = torch.randn(50, 128, device="cuda")
+logits = torch.randn(150, 9000, device="cuda")
+tokens = torch.arange(150, device="cuda")
+out = torch.empty(2, 128, device="cuda")
+torch.cuda.synchronize()
+kv.prefill(0, x, x); kv.prefill(1, x, x)
+ctx.sync()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    kv.push(x[:2], x[:2])
+    kv.attention(x[:2], out)
+    got = token_logprobs_device(ctx, logits, tokens, 3)
+graph.replay()
+torch.cuda.synchronize()
+want = torch.log_softmax(logits, -1).gather(1, tokens[:, None])[:, 0]
+assert (got.logprob - want).abs().max() < 1e-4
+assert kv.state(1) == (51, 51) and torch.isfinite(out).all()
+ctx.sync()
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "fine", r.stdout + r.stderr
+
+
+def test_in_place_and_out_of_order(ctx):
+    """The result over its own queries; sequences filled in any order; one
+    sequence emptied and filled again between steps of the others."""
+    rng = np.random.default_rng(12)
+    heads, dim = 2, 128
+    width = heads * dim
+    for tokens in (40, 9000):  # one CTA per head, and several clusters
+        kv = QuantizedKvCache(ctx, 2, heads, dim, 4, tokens, 4)
+        k, v = (dev(rng.standard_normal((tokens, width)).astype(np.float32)) for _ in range(2))
+        kv.prefill(1, k, v)
+        kv.prefill(0, k[:7], v[:7])
+        kv.push(k[:2], v[:2])
+        q = dev(rng.standard_normal((2, width)).astype(np.float32))
+        want = host(kv.attention(q))
+        assert kv.attention(q, q) is q
+        assert np.array_equal(host(q), want)
+        kv.reset(0)
+        raises("Shape", lambda: kv.push(k[:2], v[:2]))
+        kv.prefill(0, k[:33], v[:33])
+        kv.push(k[:2], v[:2])
+        assert kv.state(0) == (34, 34) and kv.state(1) == (tokens + 2, tokens + 2)
+        q = rng.standard_normal((2, width)).astype(np.float32)
+        out = host(kv.attention(dev(q)))
+        ctx.sync()
+        check_attention(kv, q, out, heads, dim, 4)
+        kv.free()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_many_heads(ctx, bits):
+    """More (key or value) rows than a push has warps."""
+    rng = np.random.default_rng(13)
+    heads, dim, batch = 37, 48, 2
+    kv, q, out = run_attention(ctx, rng, (70, 31), heads, dim, bits, 3, 5)
+    check_attention(kv, q, out, heads, dim, bits)
+    kv.free()

@@ -143,6 +143,12 @@ void launch_kvq_reset(int* state, int seq, cudaStream_t st) {
 // tokens are eight values over eight lanes: halving what a lane keeps at every
 // exchange takes 7 shuffles instead of 24 and leaves the extremes of token u in
 // the lanes u and u + 4 of the eight, which then find its parameters once.
+// Place of byte `byte` of the codes in the stage (see the stores).
+__device__ __forceinline__ int kvq_staged(int byte) {
+  const int plane = byte >> 9;
+  return byte ^ ((plane & 7) << 4) ^ ((plane & 6) << 1);
+}
+
 // VEC: rows that four floats at a time can be read from, so that a lane's four dims
 // are the row's or not as one.  (Five CTAs per SM, 48 registers: a prompt of 32,768
 // tokens takes 94 us with them, 8 bits, 107 with three and 104 with six.)
@@ -239,13 +245,19 @@ __global__ void __launch_bounds__(256, 5)
           for (int i = 0; i < 4; ++i)
             if (d0 + i >= L.dim) c[u] &= ~(0xFFu << (8 * i));
       }
+      // Word i of a lane lies at plane * 512 + (g * 4 + j) * 16 + word * 4 (kvq_key_byte,
+      // kvq_value_byte), g growing with i; in the stage the 16-byte unit's lowest three
+      // bits are xored with the plane, the word with half of it (kvq_staged): a store's
+      // lanes meet in a bank by twos instead of by eights and sixteens.
+      const int byte = part ? kvq_value_byte(half * 16 + j * 4, d0, BITS) : kvq_key_byte(warp * 4, d0, BITS);
+      unsigned char* even = codes + kvq_staged(byte);
+      unsigned char* odd_one = codes + (kvq_staged(byte) ^ 64);
       if (part == 0) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (BITS == 4) c[u] |= __shfl_xor_sync(0xffffffffu, c[u], 4) << 4;
-          c[u] ^= kvq_flip(BITS);
           if (real && (BITS == 8 || !h4))
-            *reinterpret_cast<uint32_t*>(codes + kvq_key_byte(warp * 4 + u, d0, BITS)) = c[u];
+            *reinterpret_cast<uint32_t*>((u & 1 ? odd_one : even) + (u >> 1) * 128) = c[u] ^ kvq_flip(BITS);
         }
       } else {
         // bytes: token u of dim i; as words: dim i of the four tokens
@@ -256,9 +268,8 @@ __global__ void __launch_bounds__(256, 5)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (BITS == 4) w[i] |= __shfl_xor_sync(0xffffffffu, w[i], 2) << 4;
-          w[i] ^= kvq_flip(BITS);
           if (real && (BITS == 8 || !h2))
-            *reinterpret_cast<uint32_t*>(codes + kvq_value_byte(half * 16 + j * 4, d0 + i, BITS)) = w[i];
+            *reinterpret_cast<uint32_t*>((i & 1 ? odd_one : even) + (i >> 1) * 128) = w[i] ^ kvq_flip(BITS);
         }
       }
     }
@@ -266,8 +277,18 @@ __global__ void __launch_bounds__(256, 5)
   __syncthreads();
   // (slots past the prompt's end in its last tile get zeros: nothing is in them)
   uint4* out = reinterpret_cast<uint4*>(kvq_tile(data, L, seq, h, tile * 32LL));
-  const uint4* in = reinterpret_cast<const uint4*>(kvq_stage);
-  for (int i = threadIdx.x; i < L.tile / 16; i += 256) out[i] = in[i];
+  for (int i = threadIdx.x; i < L.tile / 16; i += 256) {
+    const int at = i * 16, part = at >= L.half, byte = at - part * L.half;
+    if (byte >= L.codes) {
+      out[i] = *reinterpret_cast<const uint4*>(kvq_stage + at);
+      continue;
+    }
+    const int staged = kvq_staged(byte);  // a unit's words are permuted by their number's xor
+    uint4 w = *reinterpret_cast<const uint4*>(kvq_stage + part * L.half + (staged & ~15));
+    if (staged & 4) w = make_uint4(w.y, w.x, w.w, w.z);
+    if (staged & 8) w = make_uint4(w.z, w.w, w.x, w.y);
+    out[i] = w;
+  }
 }
 
 // Rows that four floats at a time can be read from (or written to).

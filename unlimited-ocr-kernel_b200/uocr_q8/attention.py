@@ -191,15 +191,15 @@ class KvCache:
 _FP32 = None  # torch.float32, once torch has been imported
 
 
-def _rows(t, rows, width: int, what: str):
-    """Checks [rows x width] FP32 CUDA rows (rows None: any number) and returns
-    (rows, floats between rows)."""
+def _rows(t, rows, width: int, what: str, device: int):
+    """Checks [rows x width] FP32 rows (rows None: any number) of adjacent floats
+    on CUDA device `device` and returns (rows, floats between rows)."""
     global _FP32
     if _FP32 is None:
         import torch
         _FP32 = torch.float32
     shape = t.shape
-    if len(shape) == 2 and t.dtype is _FP32 and t.is_cuda:
+    if len(shape) == 2 and t.dtype is _FP32 and t.get_device() == device:
         n, w = shape
         if w == width and (n == rows or rows is None):
             between, apart = t.stride()
@@ -208,9 +208,9 @@ def _rows(t, rows, width: int, what: str):
             if (apart == 1 or w == 1) and (between >= w or n <= 1):
                 return n, between if n > 1 else w
     from . import OcrError
-    raise OcrError(4, f"invalid tensor shape: {what}: FP32 CUDA rows "
-                      f"{['rows' if rows is None else rows, width]} of adjacent floats expected, got "
-                      f"{list(shape)} {t.dtype} on {t.device}")
+    raise OcrError(4, f"invalid tensor shape: {what}: FP32 rows "
+                      f"{['rows' if rows is None else rows, width]} of adjacent floats on cuda:{device} "
+                      f"expected, got {list(shape)} {t.dtype} on {t.device}")
 
 
 class QuantizedKvCache:
@@ -235,22 +235,22 @@ class QuantizedKvCache:
 
     def _whole(self, t, rows: int, width: int, what: str) -> int:
         """Checks contiguous rows and returns their address."""
-        if _rows(t, rows, width, what)[1] != width:
+        if _rows(t, rows, width, what, self.ctx.device)[1] != width:
             from . import OcrError
             raise OcrError(4, f"invalid tensor shape: {what}: contiguous rows expected")
         return t.data_ptr()
 
     def prefill(self, seq: int, keys_t, values_t):
         """The rows of a prompt into the empty sequence seq."""
-        tokens, ld_k = _rows(keys_t, None, self.width, "keys")
-        ld_v = _rows(values_t, tokens, self.width, "values")[1]
+        tokens, ld_k = _rows(keys_t, None, self.width, "keys", self.ctx.device)
+        ld_v = _rows(values_t, tokens, self.width, "values", self.ctx.device)[1]
         _check(self._lib.uocr_kvq_prefill(self.ctx.handle, self._h, seq, keys_t.data_ptr(), ld_k,
                                           values_t.data_ptr(), ld_v, tokens))
 
     def push(self, k_t, v_t):
         """Row b of k and v into every sequence b."""
-        ld_k = _rows(k_t, self.batch, self.width, "k")[1]
-        ld_v = _rows(v_t, self.batch, self.width, "v")[1]
+        ld_k = _rows(k_t, self.batch, self.width, "k", self.ctx.device)[1]
+        ld_v = _rows(v_t, self.batch, self.width, "v", self.ctx.device)[1]
         _check(self._lib.uocr_kvq_push(self.ctx.handle, self._h, k_t.data_ptr(), ld_k,
                                        v_t.data_ptr(), ld_v))
 

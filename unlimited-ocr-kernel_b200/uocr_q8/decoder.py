@@ -338,11 +338,12 @@ def token_logprobs_device(ctx: GpuContext, logits_t, tokens_t=None, top_k: int =
         import torch
         _INT64 = torch.int64
     rows, vocab = logits_t.shape if logits_t.dim() == 2 else (0, 0)
-    between = _rows(logits_t, rows, vocab, "logits")[1]
-    if tokens_t is not None and (tokens_t.dtype is not _INT64 or not tokens_t.is_cuda
+    between = _rows(logits_t, rows, vocab, "logits", ctx.device)[1]
+    if tokens_t is not None and (tokens_t.dtype is not _INT64 or tokens_t.get_device() != ctx.device
                                  or tokens_t.shape != (rows,) or not tokens_t.is_contiguous()):
         from . import OcrError
-        raise OcrError(4, "invalid tensor shape: tokens: contiguous int64 CUDA [rows] expected")
+        raise OcrError(4, "invalid tensor shape: tokens: contiguous int64 [rows] on "
+                          f"cuda:{ctx.device} expected")
     if top_k < 0:
         from . import OcrError
         raise OcrError(4, "invalid tensor shape: top_k must not be negative")
