@@ -325,6 +325,23 @@ __global__ void __launch_bounds__(kKvqPushWarps * 32)
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   const int b = blockIdx.x;
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7;
+  const int half = L.dim >> 1;
+  const long long width = static_cast<long long>(L.heads) * L.dim;
+  // A lane's four dims of task's row from dim d0, and what they are rotated with.
+  float x[4], y[4];
+  auto load = [&](int task, int d0) {
+    const bool value = task & 1;
+    const float* row = (value ? v + b * ld_v : k + b * ld_k) + static_cast<long long>(task >> 1) * L.dim;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = d0 + i;
+      x[i] = d < L.dim ? row[d] : 0.0f;
+      if (ROPE && !value) y[i] = d < L.dim ? row[d < half ? d + half : d - half] : 0.0f;
+    }
+  };
+  // (the first rows and the state arrive together)
+  if (warp < 2 * L.heads) load(warp, (lane >> 3) * 32 + l8 * 4);
   const int prefix = state[2 * b], gen = state[2 * b + 1];
   if (prefix <= 0) {
     if (threadIdx.x == 0) flag(status, DEV_CACHE);
@@ -333,37 +350,32 @@ __global__ void __launch_bounds__(kKvqPushWarps * 32)
   const int pos = prefix + gen;
   const long long slot = prefix + gen % window;
   const int t = static_cast<int>(slot & 31);
-  const int half = L.dim >> 1;
-  const long long width = static_cast<long long>(L.heads) * L.dim;
   const bool turn = ROPE && pos >= 0 && pos < max_pos;
   if (ROPE && !turn && threadIdx.x == 0) flag(status, DEV_POSITION);
   const float2* cs = ROPE ? table + static_cast<long long>(pos) * half : nullptr;
-  // element d of a row, rotated (one rounding per operation, as uocr_kv_rope)
-  auto rotated = [&](const float* row, int d) {
-    if (!turn) return row[d];
-    const int i = d < half ? d : d - half;
-    const float2 c = cs[i];
-    const float x0 = row[i], x1 = row[i + half];
+  // element d of a row, x0, rotated with x1, half a row from it (one rounding per
+  // operation, as uocr_kv_rope)
+  auto rotated = [&](float x0, float x1, int d) {
+    if (!turn) return x0;
+    const float2 c = cs[d < half ? d : d - half];
     return d < half ? __fsub_rn(__fmul_rn(x0, c.x), __fmul_rn(x1, c.y))
-                    : __fadd_rn(__fmul_rn(x1, c.x), __fmul_rn(x0, c.y));
+                    : __fadd_rn(__fmul_rn(x0, c.x), __fmul_rn(x1, c.y));
   };
-  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31, l8 = lane & 7;
   for (int task = warp; task < 2 * L.heads; task += warps) {
     const int h = task >> 1;
     const bool value = task & 1;
     const long long off = static_cast<long long>(h) * L.dim;
-    const float* row = (value ? v + b * ld_v : k + b * ld_k) + off;
     unsigned char* codes = kvq_tile(data, L, b, h, slot) + (value ? L.half : 0);
     for (int q = 0; q < (L.groups + 3) / 4; ++q) {
       const int grp = q * 4 + (lane >> 3), d0 = grp * 32 + l8 * 4;
       const bool real = grp < L.groups;
-      float x[4], hi = -INFINITY, neg_lo = -INFINITY;
+      if (task != warp || q) load(task, d0);
+      float hi = -INFINITY, neg_lo = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = d0 + i;
-        x[i] = 0.0f;
         if (d < L.dim) {
-          x[i] = ROPE && !value ? rotated(row, d) : row[d];
+          if (ROPE && !value) x[i] = rotated(x[i], y[i], d);
           hi = max_nan(hi, x[i]);
           neg_lo = max_nan(neg_lo, -x[i]);
         }
@@ -399,8 +411,9 @@ __global__ void __launch_bounds__(kKvqPushWarps * 32)
       }
     }
     if (ROPE && !value) {
-      const float* q = row - width;
-      for (int d = lane; d < L.dim; d += 32) q_out[b * width + off + d] = rotated(q, d);
+      const float* q = k - width + b * ld_k + off;
+      for (int d = lane; d < L.dim; d += 32)
+        q_out[b * width + off + d] = rotated(q[d], q[d < half ? d + half : d - half], d);
     }
   }
   __syncthreads();  // every thread has read `gen`
