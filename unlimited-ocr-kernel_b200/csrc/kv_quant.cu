@@ -143,6 +143,9 @@ void launch_kvq_reset(int* state, int seq, cudaStream_t st) {
 // tokens are eight values over eight lanes: halving what a lane keeps at every
 // exchange takes 7 shuffles instead of 24 and leaves the extremes of token u in
 // the lanes u and u + 4 of the eight, which then find its parameters once.
+// Bound by the bytes of the rows and, nearly as much, by issue and the latency of a
+// CTA's load - compute - copy chain: 32,768 tokens of 10 heads of 128 take 78 us in
+// 4 bits (388 MB: 5.0 TB/s) and 87 us in 8 bits (430 MB: 4.9 TB/s).
 // Place of byte `byte` of the codes in the stage (see the stores).
 __device__ __forceinline__ int kvq_staged(int byte) {
   const int plane = byte >> 9;
@@ -310,7 +313,8 @@ void launch_kvq_prefill(unsigned char* data, const KvqLayout& L, int* state, int
 }
 
 // ---- one token of every sequence ----------------------------------------------------
-// One CTA per sequence, one warp per head and key or value; lanes as above, the
+// Bound by the latency of a launch and two dependent loads (2.4 us in a chain of
+// launches, for 1 sequence as for 64).  One CTA per sequence, one warp per head and key or value; lanes as above, the
 // token's bytes straight into the tile.  ROPE: the rows are the fused projections
 // [q | k | v]; q is rotated into q_out and k rotated before it is quantised.
 constexpr int kKvqPushWarps = 20;
@@ -447,7 +451,8 @@ __device__ __forceinline__ int kvq_tokens(const int* state, int b, int window) {
 }
 
 // ---- reading back -----------------------------------------------------------------
-// Slots [first, first + count) of one sequence as token-major rows of floats: one
+// Bound by the rows written: 32,768 tokens of 10 heads of 128 take 62 us from 4 bits
+// and 71 us from 8 (6.2 and 6.1 TB/s).  Slots [first, first + count) of one sequence as token-major rows of floats: one
 // CTA per (tile, head), the tile staged in shared memory, lanes as in the prompt's
 // kernel.
 template <int BITS, bool VEC>
@@ -545,22 +550,36 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 // loop has no barrier but the ring's.  The warps' parts are joined in shared
 // memory, the CTAs' of a cluster through distributed shared memory, the clusters'
 // of a head (where the heads are few) by the one that ends last.
+//
+// Bound by the cache's bytes where there are many: 64 sequences of 2,176 tokens, 10
+// heads of 128, take 39.4 us in 4 bits (222.8 MB: 5.7 TB/s, 4 us of it the start and
+// the end of a launch) and 61.8 us in 8 bits (401 MB: 6.5 TB/s), 128 sequences of
+// 2,048 tokens 65.7 us in 4 bits (6.4 TB/s); one of 1,645 tokens takes 4.4 us, one of
+// 32,768 tokens 15 us (7 us without its bytes).  The same from dequantised values
+// would need some 3 instructions an element, a scheduler's whole rate at this
+// bandwidth; here it is about 1.6 an element (ncu: 40 % of the issue slots).
 constexpr float kLog2e = 1.44269504f;
 // Scores may pass the running maximum by this much: weights stay below 2^2.
 constexpr float kKvqSlack = 1.38f;
 constexpr int kKvqSlackBits = 2;
-constexpr int kKvqSlots = 2;  // ring slots per warp
+// Ring slots per warp.  Two tiles in flight for each of 17 warps per SM hide the
+// memory better than more for fewer warps (64 x 2,176 tokens, 4 bits: 2 slots 39.4
+// us, 3 slots 46.2, 4 slots 52.9).
+constexpr int kKvqSlots = 2;
 constexpr int kKvqCluster = 8;  // most CTAs of a cluster (portable)
 
 __host__ __device__ constexpr int kvq_tile_bytes(int groups, int bits) {
   return 2 * groups * (512 * (bits / 4) + 128);
 }
 
-// Tiles per turn of a warp and per ring slot.
+// Tiles per turn of a warp and per ring slot: two of the smallest tiles (larger ones
+// gain nothing by it: 39.9 against 39.2 us for the sizes above).
 __host__ __device__ constexpr int kvq_per(int groups, int bits) {
   return kvq_tile_bytes(groups, bits) <= 1280 ? 2 : 1;
 }
-// Warps of a CTA.
+// Warps of a CTA: about 45 KB of shared memory, so that five CTAs share an SM and
+// 740 of them, more than the 640 heads of a batch of 64, run at once (8 bits, 9 KB
+// tiles: two warps 62.4 us, four 71.8).
 __host__ __device__ constexpr int kvq_warps(int groups, int bits) {
   const int turn = kvq_tile_bytes(groups, bits) * kvq_per(groups, bits);
   return turn <= 5120 ? 4 : turn <= 10240 ? 2 : 1;
@@ -1045,7 +1064,9 @@ static cudaError_t launch_kvq_attention_t(KvqAttnArgs a, int batch, cudaStream_t
   });
   // Every CTA resident at once where the heads are few: clusters of up to eight
   // while the warps of a head outnumber no tiles of a full cache, then several
-  // clusters per head while every warp keeps 4 tiles.
+  // clusters per head while every warp keeps 4 tiles (one sequence of 32,768 tokens,
+  // 10 heads: 32 us without the second step, 17.9 with it, 22.7 where warps may keep
+  // fewer tiles and the CTAs no longer fit at once).
   constexpr int W = Shared::W;
   const long long heads = static_cast<long long>(batch) * a.layout.heads;
   constexpr int kPerSm = 227 * 1024 / (smem + 1024);
