@@ -495,12 +495,14 @@ int uocr_kv_export(uocr_ctx *ctx, const uocr_kv *kv, size_t seq, float *keys_out
  *   uocr_kvq_prefill:  the rows of a prompt into the empty sequence seq;
  *   uocr_kvq_push:     row b of k/v into every sequence b;
  *   uocr_kvq_rope, uocr_kvq_rope_push_qkv: as uocr_kv_rope and
- *                      uocr_kv_rope_push_qkv;
+ *                      uocr_kv_rope_push_qkv (q_out apart from qkv);
  *   uocr_kvq_attention: softmax(q . K / sqrt(head_dim)) V of q row b over the
  *                      tokens of sequence b and what the cache stands for, FP32
  *                      accumulation (FP32 tolerance); a row of q that is not
  *                      finite, or scores that are not, give NaN outputs for that
- *                      head and Numerical at the next synchronising call;
+ *                      head and Numerical at the next synchronising call (full
+ *                      accuracy for 32 dims of q, and for steps of the values,
+ *                      whose largest is 2^-86 and above); out may be q;
  *   uocr_kvq_read:     what slots [first, first + count) of sequence seq stand
  *                      for, as token-major rows of floats (a head's slots lie in
  *                      the physical order of uocr_kv); slots past its tokens are
@@ -537,7 +539,7 @@ int uocr_kvq_read(uocr_ctx *ctx, const uocr_kvq *kv, size_t seq, size_t first, s
  *   entropy[r]  = -sum p log p (may be NULL);
  *   top_ids / top_logprobs [rows x top_k]: the top_k largest logits, larger
  *                 first, equal ones by the lower id, and their log p
- *                 (top_k <= 32 and <= vocab; 0: none).
+ *                 (top_k <= 32 and <= vocab; 0: none; vocab <= 2^30).
  * -inf is a logit of probability 0 (a banned token).  A row that holds NaN or
  * +inf, or nothing but -inf, gives NaN (ids -1) and Numerical at the next
  * synchronising call; a token id of vocab or above NaN and Shape.  Sums in FP32,

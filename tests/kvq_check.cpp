@@ -138,7 +138,7 @@ static int refusals() {
   EXPECT(uocr_token_logprobs(&ctx, p, 1, 8, 7, t, 0, p, p, nullptr, nullptr), UOCR_ERR_SHAPE);
   EXPECT(uocr_token_logprobs(&ctx, p, 1, 8, 0, t, 9, p, p, ids, p), UOCR_ERR_SHAPE);
   EXPECT(uocr_token_logprobs(&ctx, p, 1, 64, 0, t, 33, p, p, ids, p), UOCR_ERR_UNSUPPORTED);
-  EXPECT(uocr_token_logprobs(&ctx, p, 1, size_t(1) << 31, 0, t, 0, p, p, nullptr, nullptr),
+  EXPECT(uocr_token_logprobs(&ctx, p, 1, (size_t(1) << 30) + 1, 0, t, 0, p, p, nullptr, nullptr),
          UOCR_ERR_UNSUPPORTED);
   EXPECT(uocr_token_logprobs(&ctx, p, size_t(1) << 31, 8, 0, t, 0, p, p, nullptr, nullptr),
          UOCR_ERR_UNSUPPORTED);

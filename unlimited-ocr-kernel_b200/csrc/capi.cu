@@ -2100,8 +2100,8 @@ int uocr_token_logprobs(uocr_ctx* ctx, const float* logits_dev, size_t rows, siz
   if (top_k > vocab) return fail(UOCR_ERR_SHAPE, "invalid tensor shape: more alternatives than logits");
   if (top_k > static_cast<size_t>(kLogprobMaxTop))
     return fail(UOCR_ERR_UNSUPPORTED, "unsupported configuration: more than %d alternatives", kLogprobMaxTop);
-  if (!fits_int(vocab) || !fits_int(rows) || ld >> 40)
-    return fail(UOCR_ERR_UNSUPPORTED, "unsupported configuration: logits extent above 2^31");
+  if (vocab > (size_t(1) << 30) || !fits_int(rows) || ld >> 40)
+    return fail(UOCR_ERR_UNSUPPORTED, "unsupported configuration: more than 2^30 logits or 2^31 rows");
   if ((tokens_dev == nullptr) != (logprob_dev == nullptr))
     return fail(UOCR_ERR_INVALID, "token ids and their log probabilities come together");
   if (rows == 0) return ok();

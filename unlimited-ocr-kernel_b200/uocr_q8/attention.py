@@ -188,16 +188,16 @@ class KvCache:
             pass
 
 
-_FP32 = None  # torch.float32, once torch has been imported
+_FP32 = _empty_like = None  # torch's, once it has been imported
 
 
 def _rows(t, rows, width: int, what: str, device: int):
     """Checks [rows x width] FP32 rows (rows None: any number) of adjacent floats
     on CUDA device `device` and returns (rows, floats between rows)."""
-    global _FP32
+    global _FP32, _empty_like
     if _FP32 is None:
         import torch
-        _FP32 = torch.float32
+        _FP32, _empty_like = torch.float32, torch.empty_like
     shape = t.shape
     if len(shape) == 2 and t.dtype is _FP32 and t.get_device() == device:
         n, w = shape
@@ -275,7 +275,7 @@ class QuantizedKvCache:
         """softmax(q K^T / sqrt(head_dim)) V of row b of q over sequence b."""
         q = self._whole(q_t, self.batch, self.width, "q")
         if out_t is None:
-            out_t = q_t.new_empty((self.batch, self.width))
+            out_t = _empty_like(q_t)
         else:
             self._whole(out_t, self.batch, self.width, "out")
         _check(self._lib.uocr_kvq_attention(self.ctx.handle, self._h, q, out_t.data_ptr()))
