@@ -499,8 +499,9 @@ int uocr_kv_export(uocr_ctx *ctx, const uocr_kv *kv, size_t seq, float *keys_out
  *   uocr_kvq_attention: softmax(q . K / sqrt(head_dim)) V of q row b over the
  *                      tokens of sequence b and what the cache stands for, FP32
  *                      accumulation (FP32 tolerance); a row of q that is not
- *                      finite, or scores that are not, give NaN outputs for that
- *                      head and Numerical at the next synchronising call (full
+ *                      finite (2^127 and above counts as such), or scores that are
+ *                      not, give NaN outputs for that head and Numerical at the
+ *                      next synchronising call (full
  *                      accuracy for 32 dims of q, and for steps of the values,
  *                      whose largest is 2^-86 and above); out may be q;
  *   uocr_kvq_read:     what slots [first, first + count) of sequence seq stand

@@ -317,6 +317,42 @@ def test_attention_flat_and_peaked(ctx, bits, q_size):
     kv.free()
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e12, 1e29])
+def test_attention_vast_scores(ctx, bits, size):
+    """Scores of any size, negative ones alone among them: where the largest leads by
+    more than a sum's rounding, its token takes all the weight.  (48 roundings of
+    2^-24 of a score's terms at most: 2^-18 of them; the sum to L >= 1 and the two
+    products of a value are three roundings, the weight's own 2^-30 and the least
+    value's join three more: 2^-21 of s code + |m|.)"""
+    rng = np.random.default_rng(int(np.log10(size)) + bits)
+    heads, dim, tokens = 4, 96, 300
+    kv = QuantizedKvCache(ctx, 1, heads, dim, 4, tokens, bits)
+    k, v = (rng.standard_normal((tokens, heads, dim)).astype(np.float32) for _ in range(2))
+    k *= np.float32(size)
+    q = rng.standard_normal((heads, dim)).astype(np.float32)
+    k[:, 2:] = np.abs(k[:, 2:])
+    q[2:] = -np.abs(q[2:])
+    kv.prefill(0, dev(k.reshape(tokens, -1)), dev(v.reshape(tokens, -1)))
+    out = host(kv.attention(dev(q.reshape(1, -1)))).reshape(heads, dim)
+    ctx.sync()
+    (kh, ks, km), (vh, vs, vm) = held(k, bits), held(v, bits)
+    scores = np.einsum("thd,hd->th", kh, q.astype(np.float64))
+    terms = np.einsum("thd,hd->th", (kh - km) + np.abs(km), np.abs(q.astype(np.float64)))
+    led = 0
+    for h in range(heads):
+        order = np.argsort(-scores[:, h])
+        gap = (scores[order[0], h] - scores[order[1], h]) / np.sqrt(dim)
+        if gap < 2.0 ** -17 * terms[:, h].max() / np.sqrt(dim) + 40:
+            continue
+        led += 1
+        t = order[0]
+        tol = 2.0 ** -21 * ((vh - vm) + np.abs(vm))[t, h] + tokens * np.exp(-40) * 8
+        assert np.all(np.abs(out[h] - vh[t, h]) <= tol), (h, np.max(np.abs(out[h] - vh[t, h]) / tol))
+    assert led >= 3
+    kv.free()
+
+
 @pytest.mark.parametrize("scale", [1e-25, 1e-12, 1e12])
 def test_attention_value_sizes(ctx, scale):
     """Values of any size; keys of the inverse size of the queries."""

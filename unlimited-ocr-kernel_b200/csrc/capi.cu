@@ -2047,7 +2047,9 @@ int uocr_kvq_attention(uocr_ctx* ctx, const uocr_kvq* kv, const float* q_dev, fl
   a.window = kv->window;
   a.q = q_dev;
   a.out = out_dev;
-  a.scale = 1.0f / std::sqrt(static_cast<float>(kv->layout.dim));
+  const double scale = 1.4426950408889634 / std::sqrt(static_cast<double>(kv->layout.dim));
+  a.scale = static_cast<float>(scale);
+  a.scale_rest = static_cast<float>(scale - a.scale);
   a.status = ctx->status_dev;
   a.sms = ctx->sms;
   a.partial = kv->partial;

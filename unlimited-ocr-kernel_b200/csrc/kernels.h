@@ -369,7 +369,7 @@ struct KvqAttnArgs {
   int window;
   const float* q;    // [batch][heads * dim]
   float* out;        // the same
-  float scale;       // 1 / sqrt(dim)
+  float scale, scale_rest;  // log2(e) / sqrt(dim), rounded, and what the rounding left
   unsigned* status;
   int sms;
   // heads spread over several clusters of CTAs: a part's {max, sum, values} per

@@ -533,7 +533,9 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 //
 //   scores:  rows = 16 tokens, k = the 32 dims of a group, columns = the four
 //            signed bytes of q 2^a (|q 2^a| < 2^30, a by the group's largest |q|);
-//            q . (c - C) = sum_b 256^b D_b, then s (q . (c - C)) + z sum(q);
+//            q . (c - C) = sum_b 256^b D_b, then s (q . (c - C)) + z sum(q), summed
+//            from minus the running maximum: a score that counts ends near zero and
+//            costs no rounding of its own size;
 //   values:  rows = 16 dims, k = the tile's 32 tokens, columns = the four bytes
 //            of p_t s_t 2^a (< 2^31, a by the largest s so far);
 //            o += 2^-a sum_b 256^b D_b, and p_t z_t is summed apart.
@@ -558,10 +560,13 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 // 32,768 tokens 15 us (7 us without its bytes).  The same from dequantised values
 // would need some 3 instructions an element, a scheduler's whole rate at this
 // bandwidth; here it is about 1.6 an element (ncu: 40 % of the issue slots).
-constexpr float kLog2e = 1.44269504f;
-// Scores may pass the running maximum by this much: weights stay below 2^2.
-constexpr float kKvqSlack = 1.38f;
+// Scores are in powers of two.  They may pass the running maximum by this much:
+// weights stay below 2^2.
+constexpr float kKvqSlack = 1.99f;
 constexpr int kKvqSlackBits = 2;
+// A tile whose scores lie further than this from the maximum that they were summed
+// against is summed again, unless a float at that maximum is too coarse for it.
+constexpr float kKvqFar = 8.0f, kKvqVast = 1048576.0f;
 // Ring slots per warp.  Two tiles in flight for each of 17 warps per SM hide the
 // memory better than more for fewer warps (64 x 2,176 tokens, 4 bits: 2 slots 39.4
 // us, 3 slots 46.2, 4 slots 52.9).
@@ -649,7 +654,7 @@ __device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
 // Factor that a part with maximum m and sum l takes in a whole with maximum M;
 // a part without tokens (m = -inf, l = 0) takes none.
 __device__ __forceinline__ float part_factor(float m, float l, float M) {
-  return m == -INFINITY && l == 0.0f ? 0.0f : exp2_fast((m - M) * kLog2e);
+  return m == -INFINITY && l == 0.0f ? 0.0f : exp2_fast(m - M);
 }
 
 template <int G, int BITS>
@@ -705,11 +710,13 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const int grp = 2 * p + col_group;
-    float v[8], big = 0.0f, sum = 0.0f;
+    float v[8], big = 0.0f;
+    double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int d = grp * 32 + (i >> 2) * 16 + 4 * j + (i & 3);
-      v[i] = d < a.layout.dim ? __ldg(a.q + row + d) : 0.0f;
+      const float qd = d < a.layout.dim ? __ldg(a.q + row + d) : 0.0f;
+      v[i] = fmaf(qd, a.scale_rest, qd * a.scale);  // q log2(e) / sqrt(dim)
       big = fmaxf(big, fabsf(v[i]));
       sum += v[i];
     }
@@ -735,21 +742,25 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
         qb[2 * p + c][1] = col_group == c ? hi : 0;
       }
     // for the accumulators: 2^-a (times 256^2 where the lane holds the upper two
-    // bytes) and, once, the sum; NaN and infinities of q reach the scores by it
+    // bytes) and the sum, its rounding in the other lane: where an outlying dim takes
+    // z far from zero, z sum(q) cancels against the upper bytes.  NaN and infinities
+    // of q reach the scores by the sum
     const int ea = __shfl_sync(0xffffffffu, e, acc_group * 16);
-    const float sa = __shfl_sync(0xffffffffu, sum, acc_group * 16);
+    const double sa = __shfl_sync(0xffffffffu, sum, acc_group * 16);
+    const float most = static_cast<float>(sa);
     const bool real = 2 * p + acc_group < G;
     qscale[p] = real ? __uint_as_float(static_cast<uint32_t>(min(ea, 254) - 29 - kShift + (j & 1) * 16) << 23) : 0.0f;
-    qsum[p] = real && !(j & 1) ? sa : 0.0f;
+    qsum[p] = !real ? 0.0f : j & 1 ? most : static_cast<float>(sa - most);
   }
 
-  float m = -INFINITY, l = 0.0f, middle[G], o[P][2][2];
-  uint32_t bound[G];    // largest step so far per group, as bf16 bits
+  float m = 0.0f, l = 0.0f, middle[G], o[P][2][2];
+  float start = 0.0f;  // of this lane's sums of scores: -m over the lanes of a row
+  int bound[G];  // largest step so far per group, as bf16 bits; -1 before the first turn
   float wup[G], wdown[P];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     middle[i] = 0.0f;
-    bound[i] = 0;
+    bound[i] = -1;
     wup[i] = 0.0f;
   }
 #pragma unroll
@@ -759,7 +770,8 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
   }
 
   const int t = g + 8 * j;  // the token of a tile that this lane weighs
-  for (int it = first, slot = 0, phase = 0; it < last; it += N) {
+  bool again = false;  // this turn's scores are summed a second time
+  for (int it = first, slot = 0, phase = 0; it < last;) {
     if (!__all_sync(0xffffffffu, mbar_wait_try(&sh.full[warp][slot], phase, a.status))) {
       // (a safety net: flagged) copies in flight land before the CTA ends
       for (int i = 1; i < kKvqSlots && it + i * N < last; ++i) {
@@ -773,7 +785,9 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
     }
     const unsigned char* tile = sh.ring[warp][slot];
     // ---- scores (of a tile past the warp's last: of whatever the slot holds, masked below)
-    float score[N];
+    float score[N];  // against m
+    uint32_t par[N][G];
+    bool in[N];
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const unsigned char* kt = tile + u * kTileBytes;
@@ -797,7 +811,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
         mma_s8_m16n8k32<true>(d[1][grp >> 1], lo.z, lo.w, hi.z, hi.w, qb[grp][0], qb[grp][1]);
       }
       // x[i]: this lane's part of the score of token g + 8 i
-      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float x[4] = {start, start, start, start};
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const int grp = min(2 * p + acc_group, G - 1);
@@ -814,34 +828,39 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
       // the four lanes of a row add up and lane j keeps token t = g + 8 j
       const float r0 = (j & 2 ? x[2] : x[0]) + __shfl_xor_sync(0xffffffffu, j & 2 ? x[0] : x[2], 2);
       const float r1 = (j & 2 ? x[3] : x[1]) + __shfl_xor_sync(0xffffffffu, j & 2 ? x[1] : x[3], 2);
-      score[u] = ((j & 1 ? r1 : r0) + __shfl_xor_sync(0xffffffffu, j & 1 ? r0 : r1, 1)) * a.scale;
+      score[u] = (j & 1 ? r1 : r0) + __shfl_xor_sync(0xffffffffu, j & 1 ? r0 : r1, 1);
     }
     // ---- the steps and least values of the tokens that are there
-    uint32_t par[N][G];
-    bool in[N], over = false;
+    bool over = false;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       in[u] = (it + u) * 32 + t < end;
-      over |= in[u] && score[u] > m + kKvqSlack;
+      over |= in[u] && score[u] > kKvqSlack;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         par[u][i] = in[u] ? *reinterpret_cast<const uint32_t*>(tile + u * kTileBytes + kTileBytes / 2 +
                                                                kCodes + i * 128 + lane * 4)
                           : 0;
-        over |= (par[u][i] & 0xFFFFu) > bound[i];
+        over |= static_cast<int>(par[u][i] & 0xFFFFu) > bound[i];
       }
     }
-    // ---- softmax: m, the maximum that the weights refer to, is raised only when
-    // a score passes it by kKvqSlack, the bounds only when a step passes them:
+    // ---- softmax: m, the maximum that scores and weights refer to, is raised only
+    // when a score passes it by kKvqSlack, the bounds only when a step passes them:
     // one vote for all in most turns
     if (__any_sync(0xffffffffu, over)) {
       float top = -INFINITY;
 #pragma unroll
       for (int u = 0; u < N; ++u) top = fmaxf(top, in[u] ? score[u] : -INFINITY);
       top = warp_max(top);
-      if (top > m) {
-        const float keep = exp2_fast((m - top) * kLog2e);
-        m = top;
+      float raise = 0.0f;
+      if (top > 0.0f || it == first) {
+        const float old = m;
+        m = old + top;
+        // (2^20 and above, where a place of m is 1/8 and more: against this tile's top,
+        // so that it weighs 1 whatever m was rounded to)
+        raise = fabsf(m) < kKvqVast ? m - old : top;
+        start = j & 1 ? -0.5f * m : 0.0f;
+        const float keep = it == first ? 0.0f : exp2_fast(-raise);
         l *= keep;
 #pragma unroll
         for (int i = 0; i < G; ++i) middle[i] *= keep;
@@ -858,21 +877,28 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
         uint32_t big = 0;
 #pragma unroll
         for (int u = 0; u < N; ++u) big = max(big, par[u][i] & 0xFFFFu);
-        bound[i] = max(bound[i], __reduce_max_sync(0xffffffffu, big));
-        // step < 2^(e - 126), weight < 2^6; steps below 2^-86 lose precision
-        const uint32_t e = max(bound[i] >> 7, 40u);
-        wup[i] = __uint_as_float((284u - kKvqSlackBits - e) << 23);
+        bound[i] = max(bound[i], static_cast<int>(__reduce_max_sync(0xffffffffu, big)));
+        // step < 2^(e - 126), weight < 2^2; steps below 2^-86 lose precision
+        const int e = max(bound[i] >> 7, 40);
+        wup[i] = __uint_as_float(static_cast<uint32_t>(284 - kKvqSlackBits - e) << 23);
       }
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        const uint32_t bd = acc_group && 2 * p + 1 < G ? bound[min(2 * p + 1, G - 1)] : bound[2 * p];
-        wdown[p] = __uint_as_float((max(bd >> 7, 40u) - 30u - kShift + kKvqSlackBits + (j & 1) * 16u) << 23);
+        const int bd = acc_group && 2 * p + 1 < G ? bound[min(2 * p + 1, G - 1)] : bound[2 * p];
+        wdown[p] = __uint_as_float(static_cast<uint32_t>(max(bd >> 7, 40) - 30 - kShift + kKvqSlackBits + (j & 1) * 16) << 23);
       }
+      if (fabsf(raise) > kKvqFar && fabsf(m) < kKvqVast && !again) {
+        again = true;
+        continue;
+      }
+#pragma unroll
+      for (int u = 0; u < N; ++u) score[u] -= raise;
     }
+    again = false;
     // ---- the weights' bytes
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const float pr = in[u] ? exp2_fast((score[u] - m) * kLog2e) : 0.0f;
+      const float pr = in[u] ? exp2_fast(score[u]) : 0.0f;
       l += pr;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
@@ -927,6 +953,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
       slot = 0;
       phase ^= 1;
     }
+    it += N;
   }
 
   // The next kernel (usually a push) may become resident now: earlier, its CTAs
@@ -949,7 +976,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
           sh.o[warp][(2 * p + acc_group) * 32 + mb * 16 + up * 8 + g] = v + add;
       }
   if (lane == 0) {
-    sh.m[warp] = m;
+    sh.m[warp] = first < last ? m : -INFINITY;
     sh.l[warp] = l;
   }
   __syncthreads();
