@@ -56,6 +56,11 @@ __device__ __forceinline__ float min3_nan(float a, float b, float c) {
   asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {  // of magnitudes; NaN is none
+  float d;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -71,20 +76,18 @@ __device__ __forceinline__ bool kvq_refused(float hi, float neg_lo) {
 constexpr float kKvqTinyStep = 1e-30f;  // steps below it (0 among them) go by double
 
 // Codes of four values as the bytes of a word: in float, rounded by adding
-// 1.5 2^23 (whose last place is 1).  *near is how far the quotients are from their
-// codes.  The float quotient is off by four roundings of 2^-24 at most, so by 6.1e-5
-// at 255 and 3.6e-6 at 15: from kvq_near on it is too near a border between two
+// 1.5 2^23 (whose last place is 1).  *near is raised to how far the quotients are from
+// their codes.  The float quotient is off by four roundings of 2^-24 at most, so by
+// 6.1e-5 at 255 and 3.6e-6 at 15: from kvq_near on it is too near a border between two
 // codes to decide.
 constexpr float kvq_near(int bits) { return bits == 4 ? 0.499995f : 0.49993f; }
 __device__ __forceinline__ uint32_t kvq_codes4(const float (&x)[4], float m, float inv_s, float* near) {
   const float2 nm = make_float2(-m, -m), is = make_float2(inv_s, inv_s);
-  const float2 magic = make_float2(12582912.0f, 12582912.0f), back = make_float2(-12582912.0f, -12582912.0f);
-  const float2 t0 = f2_mul(f2_add(make_float2(x[0], x[1]), nm), is);
-  const float2 t1 = f2_mul(f2_add(make_float2(x[2], x[3]), nm), is);
-  const float2 r0 = f2_add(t0, magic), r1 = f2_add(t1, magic);
-  const float2 o0 = f2_fma(f2_add(r0, back), make_float2(-1.0f, -1.0f), t0);
-  const float2 o1 = f2_fma(f2_add(r1, back), make_float2(-1.0f, -1.0f), t1);
-  *near = fmaxf(fmaxf(fabsf(o0.x), fabsf(o0.y)), fmaxf(fabsf(o1.x), fabsf(o1.y)));
+  const float2 magic = make_float2(12582912.0f, 12582912.0f), one = make_float2(-1.0f, -1.0f);
+  const float2 d0 = f2_add(make_float2(x[0], x[1]), nm), d1 = f2_add(make_float2(x[2], x[3]), nm);
+  const float2 r0 = f2_fma(d0, is, magic), r1 = f2_fma(d1, is, magic);
+  const float2 o0 = f2_fma(d0, is, f2_fma(r0, one, magic)), o1 = f2_fma(d1, is, f2_fma(r1, one, magic));
+  *near = max3_abs(max3_abs(*near, o0.x, o0.y), o1.x, o1.y);
   return __byte_perm(__byte_perm(__float_as_uint(r0.x), __float_as_uint(r0.y), 0x0040),
                      __byte_perm(__float_as_uint(r1.x), __float_as_uint(r1.y), 0x0040), 0x5410);
 }
@@ -178,13 +181,13 @@ __global__ void __launch_bounds__(256, 5)
     const bool real = grp < L.groups;
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-      const float* rows = (part ? v : k) + static_cast<long long>(h) * L.dim;
       const long long ld = part ? ld_v : ld_k;
+      const float* row = (part ? v : k) + t0 * ld + static_cast<long long>(h) * L.dim;
       float x[4][4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 4; ++u, row += ld) {
         if (t0 + u < tokens) {
-          kvq_load4<VEC>(rows + (t0 + u) * ld, d0, L.dim, x[u]);
+          kvq_load4<VEC>(row, d0, L.dim, x[u]);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[u][i] = 0.0f;
@@ -226,21 +229,25 @@ __global__ void __launch_bounds__(256, 5)
       if (real && l8 < 4)
         *reinterpret_cast<uint32_t*>(codes + L.codes + kvq_param_byte(warp * 4 + l8, grp)) = word;
       uint32_t c[4];
-      const bool odd = real && (s < kKvqTinyStep || lost);
+      float near = 0.0f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int from = (lane & 24) + u;
-        const float mu = __shfl_sync(0xffffffffu, m, from);
-        float near;
-        c[u] = kvq_codes4(x[u], mu, __shfl_sync(0xffffffffu, inv_s, from), &near);
-        if (__any_sync(0xffffffffu, near >= kvq_near(BITS) || (odd && (l8 & 3) == u))) {
-          const float su = __shfl_sync(0xffffffffu, s, from);
+      for (int u = 0; u < 4; ++u)
+        c[u] = kvq_codes4(x[u], __shfl_sync(0xffffffffu, m, (lane & 24) + u),
+                          __shfl_sync(0xffffffffu, inv_s, (lane & 24) + u), &near);
+      // (rare: some 7 warps in 100 at 8 bits)
+      if (__any_sync(0xffffffffu, near >= kvq_near(BITS) || s < kKvqTinyStep || lost)) {
+        if (lost) flag(status, DEV_KV_RANGE);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int from = (lane & 24) + u;
+          const float mu = __shfl_sync(0xffffffffu, m, from), su = __shfl_sync(0xffffffffu, s, from);
+          near = 0.0f;
+          c[u] = kvq_codes4(x[u], mu, __shfl_sync(0xffffffffu, inv_s, from), &near);
           if (near >= kvq_near(BITS) || su < kKvqTinyStep)
             c[u] = kvq_codes4_exactly(x[u][0], x[u][1], x[u][2], x[u][3], mu, su, levels);
           if (__shfl_sync(0xffffffffu, lost, from)) c[u] = 0;
         }
       }
-      if (lost) flag(status, DEV_KV_RANGE);
       if (d0 + 3 >= L.dim) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
@@ -389,7 +396,7 @@ __global__ void __launch_bounds__(kKvqPushWarps * 32)
         hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         neg_lo = max_nan(neg_lo, __shfl_xor_sync(0xffffffffu, neg_lo, o));
       }
-      float s, m, near;
+      float s, m, near = 0.0f;
       uint32_t word = kvq_params(-neg_lo, hi, 1.0 / levels, levels, &s, &m);
       uint32_t c = kvq_codes4(x, m, rcp_fast(s), &near);
       if (near >= kvq_near(BITS) || s < kKvqTinyStep) c = kvq_codes4_exactly(x[0], x[1], x[2], x[3], m, s, levels);
