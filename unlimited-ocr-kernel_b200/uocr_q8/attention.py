@@ -19,6 +19,7 @@ Every call goes to the CUDA library (libuocr_q8.so).
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 from . import GpuContext, Int8Matrix, QuantizationMode, _check, _tptr, lib
@@ -308,11 +309,12 @@ class QuantizedKvCache:
         return keys_t, values_t
 
     def _new(self, rows: int):
-        like = getattr(self, "_like", None)
-        if like is None:
+        make = getattr(self, "_make", None)
+        if make is None:
             import torch
-            like = self._like = torch.empty(0, dtype=torch.float32, device=f"cuda:{self.ctx.device}")
-        return like.new_empty((rows, self.width))
+            make = self._make = functools.partial(torch.empty_strided, dtype=torch.float32,
+                                                  device=torch.device("cuda", self.ctx.device))
+        return make((rows, self.width), (self.width, 1))
 
     def export(self, seq: int):
         """``read`` of every token of sequence seq (synchronous)."""

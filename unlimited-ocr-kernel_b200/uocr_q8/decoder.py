@@ -315,7 +315,7 @@ def logits_checksum_device(ctx: GpuContext, logits_t, acc_t):
     _check(lib().uocr_bits_checksum(ctx.handle, _p(logits_t), logits_t.numel(), _p(acc_t)))
 
 
-_INT64 = _empty_like = None  # torch's, once it has been imported
+_INT64 = _FP32 = _empty_strided = None  # torch's, once it has been imported
 
 
 class TokenLogprobs(NamedTuple):
@@ -333,10 +333,10 @@ def token_logprobs_device(ctx: GpuContext, logits_t, tokens_t=None, top_k: int =
     under the rows of logits_t [rows x vocab] (FP32, rows may lie apart), the
     rows' entropies and top_k most probable tokens, equal ones by the lower id
     (uocr_token_logprobs).  -inf bans a token.  Asynchronous."""
-    global _INT64, _empty_like
+    global _INT64, _FP32, _empty_strided
     if _INT64 is None:
         import torch
-        _INT64, _empty_like = torch.int64, torch.empty_like
+        _INT64, _FP32, _empty_strided = torch.int64, torch.float32, torch.empty_strided
     rows, vocab = logits_t.shape if logits_t.dim() == 2 else (0, 0)
     between = _rows(logits_t, rows, vocab, "logits", ctx.device)[1]
     if tokens_t is not None and (tokens_t.dtype is not _INT64 or tokens_t.get_device() != ctx.device
@@ -347,10 +347,11 @@ def token_logprobs_device(ctx: GpuContext, logits_t, tokens_t=None, top_k: int =
     if top_k < 0:
         from . import OcrError
         raise OcrError(4, "invalid tensor shape: top_k must not be negative")
-    new = logits_t.new_empty
-    logprob = new((rows,)) if tokens_t is not None else None
-    entropy = _empty_like(logprob) if logprob is not None else new((rows,))
-    ids, logprobs = new((rows, top_k), dtype=_INT64), new((rows, top_k))
+    device, new = logits_t.device, _empty_strided
+    logprob = new((rows,), (1,), dtype=_FP32, device=device) if tokens_t is not None else None
+    entropy = new((rows,), (1,), dtype=_FP32, device=device)
+    ids = new((rows, top_k), (top_k, 1), dtype=_INT64, device=device)
+    logprobs = new((rows, top_k), (top_k, 1), dtype=_FP32, device=device)
     _check(lib().uocr_token_logprobs(
         ctx.handle, logits_t.data_ptr(), rows, vocab, between,
         tokens_t.data_ptr() if tokens_t is not None else None, top_k,
