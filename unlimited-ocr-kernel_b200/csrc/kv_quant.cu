@@ -146,9 +146,11 @@ void launch_kvq_reset(int* state, int seq, cudaStream_t st) {
 // tokens are eight values over eight lanes: halving what a lane keeps at every
 // exchange takes 7 shuffles instead of 24 and leaves the extremes of token u in
 // the lanes u and u + 4 of the eight, which then find its parameters once.
-// Bound by the bytes of the rows and, nearly as much, by issue and the latency of a
-// CTA's load - compute - copy chain: 32,768 tokens of 10 heads of 128 take 78 us in
-// 4 bits (388 MB: 5.0 TB/s) and 87 us in 8 bits (430 MB: 4.9 TB/s).
+// Bound by the bytes of the rows and, nearly as much, by issue (0.7 of the slots) and
+// the latency of a CTA's load - compute - copy chain: 32,768 tokens of 10 heads of 128
+// take 78 us in 4 bits (388 MB: 5.0 TB/s) and 87 us in 8 bits (430 MB: 4.9 TB/s), the
+// reset before it counted in.  Persistent CTAs whose rows arrive by asynchronous copies
+// while they work on the last ones took 90 and 104 us.
 // Place of byte `byte` of the codes in the stage (see the stores).
 __device__ __forceinline__ int kvq_staged(int byte) {
   const int plane = byte >> 9;
@@ -320,10 +322,11 @@ void launch_kvq_prefill(unsigned char* data, const KvqLayout& L, int* state, int
 }
 
 // ---- one token of every sequence ----------------------------------------------------
-// Bound by the latency of a launch and two dependent loads (2.4 us in a chain of
-// launches, for 1 sequence as for 64).  One CTA per sequence, one warp per head and key or value; lanes as above, the
-// token's bytes straight into the tile.  ROPE: the rows are the fused projections
-// [q | k | v]; q is rotated into q_out and k rotated before it is quantised.
+// One CTA per sequence, one warp per head and key or value; lanes as above, the token's
+// bytes straight into the tile.  ROPE: the rows are the fused projections [q | k | v];
+// q is rotated into q_out and k rotated before it is quantised.  Bound by the latency
+// of a launch and two dependent loads: 2.4 us in a chain of launches, for 1 sequence as
+// for 64.
 constexpr int kKvqPushWarps = 20;
 
 template <int BITS, bool ROPE>
@@ -458,10 +461,10 @@ __device__ __forceinline__ int kvq_tokens(const int* state, int b, int window) {
 }
 
 // ---- reading back -----------------------------------------------------------------
+// Slots [first, first + count) of one sequence as token-major rows of floats: one CTA
+// per (tile, head), the tile staged in shared memory, lanes as in the prompt's kernel.
 // Bound by the rows written: 32,768 tokens of 10 heads of 128 take 62 us from 4 bits
-// and 71 us from 8 (6.2 and 6.1 TB/s).  Slots [first, first + count) of one sequence as token-major rows of floats: one
-// CTA per (tile, head), the tile staged in shared memory, lanes as in the prompt's
-// kernel.
+// and 71 us from 8 (6.2 and 6.1 TB/s).
 template <int BITS, bool VEC>
 __global__ void __launch_bounds__(256)
     kvq_read_kernel(const unsigned char* __restrict__ data, const KvqLayout L,
@@ -561,10 +564,10 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 // of a head (where the heads are few) by the one that ends last.
 //
 // Bound by the cache's bytes where there are many: 64 sequences of 2,176 tokens, 10
-// heads of 128, take 39.4 us in 4 bits (222.8 MB: 5.7 TB/s, 4 us of it the start and
-// the end of a launch) and 61.8 us in 8 bits (401 MB: 6.5 TB/s), 128 sequences of
-// 2,048 tokens 65.7 us in 4 bits (6.4 TB/s); one of 1,645 tokens takes 4.4 us, one of
-// 32,768 tokens 15 us (7 us without its bytes).  The same from dequantised values
+// heads of 128, take 39.3 us in 4 bits (222.8 MB: 5.7 TB/s, 4 us of it the start and
+// the end of a launch) and 62.2 us in 8 bits (401 MB: 6.5 TB/s), 128 sequences of
+// 2,048 tokens 65.7 us in 4 bits (6.4 TB/s); one of 1,645 tokens takes 5.3 us, one of
+// 32,768 tokens 15.4 us (7 us without its bytes).  The same from dequantised values
 // would need some 3 instructions an element, a scheduler's whole rate at this
 // bandwidth; here it is about 1.6 an element (ncu: 40 % of the issue slots).
 // Scores are in powers of two.  They may pass the running maximum by this much:
