@@ -569,7 +569,7 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 // 2,048 tokens 65.7 us in 4 bits (6.4 TB/s); one of 1,645 tokens takes 5.3 us, one of
 // 32,768 tokens 15.4 us (7 us without its bytes).  The same from dequantised values
 // would need some 3 instructions an element, a scheduler's whole rate at this
-// bandwidth; here it is about 1.6 an element (ncu: 40 % of the issue slots).
+// bandwidth; here it is about 1.8 an element (ncu: 54 % of the issue slots).
 // Scores are in powers of two.  They may pass the running maximum by this much:
 // weights stay below 2^2.
 constexpr float kKvqSlack = 1.99f;
