@@ -149,6 +149,24 @@ def test_values_read_back(ctx, bits, kind):
     kv.free()
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [33, 37, 65, 97])
+def test_one_small_step_beside_others(ctx, bits, dim):
+    """A group of few dims whose step is far below every other token's."""
+    rng = np.random.default_rng(dim + bits)
+    x = rng.standard_normal((64, 1, dim)).astype(np.float32)
+    for t in range(64):
+        if t % 4 == (t // 4) % 4:
+            x[t, :, dim // 32 * 32:] = np.float32(2.0 ** -100) * (1 + np.arange(1, dim % 32 + 1) * np.float32(2.0 ** -10))
+    rows = dev(x.reshape(64, -1))
+    kv = QuantizedKvCache(ctx, 1, 1, dim, 1, 64, bits)
+    kv.prefill(0, rows, rows)
+    for got in kv.read(0, 0, 64):
+        ctx.sync()
+        assert np.array_equal(host(got), held(x, bits)[0].reshape(64, -1).astype(np.float32))
+    kv.free()
+
+
 def test_storage_bytes(ctx):
     """bits + 1 bits a dim at whole groups, in whole tiles of 32 tokens."""
     for bits in (4, 8):

@@ -39,10 +39,12 @@ __device__ __forceinline__ uint32_t kvq_params(float lo, float hi, double inv_le
   return (sb >> 16) | mb;
 }
 
-__device__ __forceinline__ float rcp_fast(float x) {  // 1 ulp; subnormals count as 0
+// 1 / x within 2^-24 of it: one step of Newton's from an approximation (1 ulp);
+// subnormals count as 0.
+__device__ __forceinline__ float rcp_fast(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+  return __fmaf_rn(__fmaf_rn(-x, y, 1.0f), y, y);
 }
 
 // Largest and least of three and of two; NaN where one is.
@@ -77,10 +79,10 @@ constexpr float kKvqTinyStep = 1e-30f;  // steps below it (0 among them) go by d
 
 // Codes of four values as the bytes of a word: in float, rounded by adding
 // 1.5 2^23 (whose last place is 1).  *near is raised to how far the quotients are from
-// their codes.  The float quotient is off by four roundings of 2^-24 at most, so by
-// 6.1e-5 at 255 and 3.6e-6 at 15: from kvq_near on it is too near a border between two
-// codes to decide.
-constexpr float kvq_near(int bits) { return bits == 4 ? 0.499995f : 0.49993f; }
+// their codes.  The float quotient is off by the roundings of the difference and of
+// the reciprocal, 2^-23 of it (and a place of the rest, 2^-26), so by 3.1e-5 at 255 and
+// 1.9e-6 at 15: from kvq_near on it is too near a border between two codes to decide.
+constexpr float kvq_near(int bits) { return bits == 4 ? 0.499998f : 0.499969f; }
 __device__ __forceinline__ uint32_t kvq_codes4(const float (&x)[4], float m, float inv_s, float* near) {
   const float2 nm = make_float2(-m, -m), is = make_float2(inv_s, inv_s);
   const float2 magic = make_float2(12582912.0f, 12582912.0f), one = make_float2(-1.0f, -1.0f);
@@ -92,12 +94,13 @@ __device__ __forceinline__ uint32_t kvq_codes4(const float (&x)[4], float m, flo
                      __byte_perm(__float_as_uint(r1.x), __float_as_uint(r1.y), 0x0040), 0x5410);
 }
 
-// The same by the definition, in double.
+// The same by the definition, in double (the four divisions in step: a warp that comes
+// here holds up its CTA; one by one they cost 2 us of 78).
 __device__ __noinline__ uint32_t kvq_codes4_exactly(float x0, float x1, float x2, float x3, float m,
                                                     float s, int levels) {
   const float x[4] = {x0, x1, x2, x3};
   uint32_t c = 0;
-#pragma unroll 1
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
     int v = 0;
     if (s > 0.0f)
@@ -140,32 +143,27 @@ void launch_kvq_reset(int* state, int seq, cudaStream_t st) {
 }
 
 // ---- a prompt's rows ------------------------------------------------------------
-// One CTA per (tile, head), one warp per four neighbouring tokens, so that the
-// bytes of a value word (four tokens of one dim) meet in one lane.  Eight lanes
-// share a group, four dims each; four groups at a time.  The extremes of four
-// tokens are eight values over eight lanes: halving what a lane keeps at every
-// exchange takes 7 shuffles instead of 24 and leaves the extremes of token u in
-// the lanes u and u + 4 of the eight, which then find its parameters once.
-// Bound by the bytes of the rows and, nearly as much, by issue (0.7 of the slots) and
-// the latency of a CTA's load - compute - copy chain: 32,768 tokens of 10 heads of 128
-// take 78 us in 4 bits (388 MB: 5.0 TB/s) and 87 us in 8 bits (430 MB: 4.9 TB/s), the
-// reset before it counted in.  Persistent CTAs whose rows arrive by asynchronous copies
-// while they work on the last ones took 90 and 104 us.
-// Place of byte `byte` of the codes in the stage (see the stores).
-__device__ __forceinline__ int kvq_staged(int byte) {
-  const int plane = byte >> 9;
-  return byte ^ ((plane & 7) << 4) ^ ((plane & 6) << 1);
-}
-
+// One CTA per (tile, head), one warp per four tokens: of the keys every eighth, whose
+// codes are one 16-byte unit of a plane, of the values neighbours, so that the bytes of
+// a value word (four tokens of one dim) meet in one lane.  Eight lanes share a group,
+// four dims each; four groups at a time.  The extremes of four tokens are eight values
+// over eight lanes: halving what a lane keeps at every exchange takes 7 shuffles instead
+// of 24 and leaves the extremes of token u in the lanes u and u + 4 of the eight, which
+// then find its parameters once.
+// Bound by the bytes of the rows and, nearly as much, by issue and the latency of a
+// CTA's load - compute - copy chain: 32,768 tokens of 10 heads of 128 take 70.6 us in 4
+// bits (388 MB: 5.5 TB/s) and 74.3 us in 8 bits (430 MB: 5.8 TB/s), the reset before it
+// counted in.  Persistent CTAs whose rows arrive by asynchronous copies while they work
+// on the last ones were slower (104 against 87 us).
 // VEC: rows that four floats at a time can be read from, so that a lane's four dims
-// are the row's or not as one.  (Five CTAs per SM, 48 registers: a prompt of 32,768
-// tokens takes 94 us with them, 8 bits, 107 with three and 104 with six.)
+// are the row's or not as one.  (Six CTAs per SM, 40 registers; with five 79 us instead
+// of 78, 8 bits, before the last two steps.)
 template <int BITS, bool VEC>
-__global__ void __launch_bounds__(256, 5)
+__global__ void __launch_bounds__(256, 6)
     kvq_prefill_kernel(unsigned char* data, const KvqLayout L, int* state, int seq,
                        const float* __restrict__ k, long long ld_k, const float* __restrict__ v,
                        long long ld_v, int tokens, unsigned* status) {
-  extern __shared__ __align__(16) unsigned char kvq_stage[];
+  extern __shared__ __align__(128) unsigned char kvq_stage[];
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   constexpr int levels = (1 << BITS) - 1;
@@ -175,7 +173,6 @@ __global__ void __launch_bounds__(256, 5)
     state[2 * seq] = tokens;
     state[2 * seq + 1] = 0;
   }
-  const int t0 = tile * 32 + warp * 4;  // this warp's tokens: t0 .. t0 + 3
   const int half = warp >> 2, j = warp & 3;
   const bool h4 = l8 & 4, h2 = l8 & 2, h1 = l8 & 1;
   for (int q = 0; q < (L.groups + 3) / 4; ++q) {
@@ -183,12 +180,15 @@ __global__ void __launch_bounds__(256, 5)
     const bool real = grp < L.groups;
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
+      // this warp's tokens: for keys each eighth, so that they are one 16-byte unit, for
+      // values neighbours, the bytes of a word
+      const int first = tile * 32 + (part ? warp * 4 : warp), step = part ? 1 : 8;
       const long long ld = part ? ld_v : ld_k;
-      const float* row = (part ? v : k) + t0 * ld + static_cast<long long>(h) * L.dim;
+      const float* row = (part ? v : k) + first * ld + static_cast<long long>(h) * L.dim;
       float x[4][4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u, row += ld) {
-        if (t0 + u < tokens) {
+      for (int u = 0; u < 4; ++u, row += step * ld) {
+        if (first + step * u < tokens) {
           kvq_load4<VEC>(row, d0, L.dim, x[u]);
         } else {
 #pragma unroll
@@ -229,15 +229,16 @@ __global__ void __launch_bounds__(256, 5)
       if (lost) word = 0x7FC00000u;
       unsigned char* codes = kvq_stage + part * L.half;
       if (real && l8 < 4)
-        *reinterpret_cast<uint32_t*>(codes + L.codes + kvq_param_byte(warp * 4 + l8, grp)) = word;
+        *reinterpret_cast<uint32_t*>(codes + L.codes + kvq_param_byte(part ? warp * 4 + l8 : warp + 8 * l8, grp)) = word;
       uint32_t c[4];
       float near = 0.0f;
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         c[u] = kvq_codes4(x[u], __shfl_sync(0xffffffffu, m, (lane & 24) + u),
                           __shfl_sync(0xffffffffu, inv_s, (lane & 24) + u), &near);
-      // (rare: some 7 warps in 100 at 8 bits)
-      if (__any_sync(0xffffffffu, near >= kvq_near(BITS) || s < kKvqTinyStep || lost)) {
+      // (rare: 3 warps in 100 at 8 bits)
+      const bool some = d0 < L.dim;
+      if (__any_sync(0xffffffffu, (some && near >= kvq_near(BITS)) || (real && s < kKvqTinyStep) || lost)) {
         if (lost) flag(status, DEV_KV_RANGE);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(256, 5)
           const float mu = __shfl_sync(0xffffffffu, m, from), su = __shfl_sync(0xffffffffu, s, from);
           near = 0.0f;
           c[u] = kvq_codes4(x[u], mu, __shfl_sync(0xffffffffu, inv_s, from), &near);
-          if (near >= kvq_near(BITS) || su < kKvqTinyStep)
+          if (some && (near >= kvq_near(BITS) || su < kKvqTinyStep))
             c[u] = kvq_codes4_exactly(x[u][0], x[u][1], x[u][2], x[u][3], mu, su, levels);
           if (__shfl_sync(0xffffffffu, lost, from)) c[u] = 0;
         }
@@ -257,20 +258,14 @@ __global__ void __launch_bounds__(256, 5)
           for (int i = 0; i < 4; ++i)
             if (d0 + i >= L.dim) c[u] &= ~(0xFFu << (8 * i));
       }
-      // Word i of a lane lies at plane * 512 + (g * 4 + j) * 16 + word * 4 (kvq_key_byte,
-      // kvq_value_byte), g growing with i; in the stage the 16-byte unit's lowest three
-      // bits are xored with the plane, the word with half of it (kvq_staged): a store's
-      // lanes meet in a bank by twos instead of by eights and sixteens.
-      const int byte = part ? kvq_value_byte(half * 16 + j * 4, d0, BITS) : kvq_key_byte(warp * 4, d0, BITS);
-      unsigned char* even = codes + kvq_staged(byte);
-      unsigned char* odd_one = codes + (kvq_staged(byte) ^ 64);
       if (part == 0) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (BITS == 4) c[u] |= __shfl_xor_sync(0xffffffffu, c[u], 4) << 4;
-          if (real && (BITS == 8 || !h4))
-            *reinterpret_cast<uint32_t*>((u & 1 ? odd_one : even) + (u >> 1) * 128) = c[u] ^ kvq_flip(BITS);
+          c[u] ^= kvq_flip(BITS);
         }
+        if (real && (BITS == 8 || !h4))
+          *reinterpret_cast<uint4*>(codes + kvq_key_byte(warp, d0, BITS)) = make_uint4(c[0], c[1], c[2], c[3]);
       } else {
         // bytes: token u of dim i; as words: dim i of the four tokens
         const uint32_t lo = __byte_perm(c[0], c[1], 0x5140), hi = __byte_perm(c[0], c[1], 0x7362);
@@ -280,26 +275,31 @@ __global__ void __launch_bounds__(256, 5)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (BITS == 4) w[i] |= __shfl_xor_sync(0xffffffffu, w[i], 2) << 4;
-          if (real && (BITS == 8 || !h2))
-            *reinterpret_cast<uint32_t*>((i & 1 ? odd_one : even) + (i >> 1) * 128) = w[i] ^ kvq_flip(BITS);
+          w[i] ^= kvq_flip(BITS);
+        }
+        // (word i lies 64 i bytes from the first: half of the lanes of a bank take them in
+        // another order, 83 -> 79 us)
+        const bool turn = lane & 8;
+        unsigned char* at = codes + kvq_value_byte(half * 16 + j * 4, d0, BITS);
+        if (real && (BITS == 8 || !h2)) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint32_t*>(at + (turn ? (i ^ 1) * 64 : i * 64)) = turn ? w[i ^ 1] : w[i];
         }
       }
     }
   }
+  // the tile leaves as one bulk copy (by vector stores of all threads 87 us, not 79)
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
   // (slots past the prompt's end in its last tile get zeros: nothing is in them)
-  uint4* out = reinterpret_cast<uint4*>(kvq_tile(data, L, seq, h, tile * 32LL));
-  for (int i = threadIdx.x; i < L.tile / 16; i += 256) {
-    const int at = i * 16, part = at >= L.half, byte = at - part * L.half;
-    if (byte >= L.codes) {
-      out[i] = *reinterpret_cast<const uint4*>(kvq_stage + at);
-      continue;
-    }
-    const int staged = kvq_staged(byte);  // a unit's words are permuted by their number's xor
-    uint4 w = *reinterpret_cast<const uint4*>(kvq_stage + part * L.half + (staged & ~15));
-    if (staged & 4) w = make_uint4(w.y, w.x, w.w, w.z);
-    if (staged & 8) w = make_uint4(w.z, w.w, w.x, w.y);
-    out[i] = w;
+  if (threadIdx.x == 0) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                     kvq_tile(data, L, seq, h, tile * 32LL)),
+                 "r"(smem_addr(kvq_stage)), "r"(static_cast<uint32_t>(L.tile))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 }
 
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(256)
     kvq_read_kernel(const unsigned char* __restrict__ data, const KvqLayout L,
                     const int* __restrict__ state, int window, int seq, long long first,
                     long long count, float* k, float* v, unsigned* status) {
-  extern __shared__ __align__(16) unsigned char kvq_stage[];
+  extern __shared__ __align__(128) unsigned char kvq_stage[];
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   const int h = blockIdx.x % L.heads;
