@@ -464,9 +464,9 @@ __device__ __forceinline__ int kvq_tokens(const int* state, int b, int window) {
 // Slots [first, first + count) of one sequence as token-major rows of floats: one CTA
 // per (tile, head), the tile staged in shared memory, lanes as in the prompt's kernel.
 // Bound by the rows written: 32,768 tokens of 10 heads of 128 take 62 us from 4 bits
-// and 71 us from 8 (6.2 and 6.1 TB/s).
+// and 69 us from 8 (6.2 and 6.3 TB/s; five CTAs per SM 62 and 71, eight 64 and 73).
 template <int BITS, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
     kvq_read_kernel(const unsigned char* __restrict__ data, const KvqLayout L,
                     const int* __restrict__ state, int window, int seq, long long first,
                     long long count, float* k, float* v, unsigned* status) {
