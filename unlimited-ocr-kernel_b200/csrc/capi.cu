@@ -1905,13 +1905,15 @@ int uocr_kvq_create(uocr_ctx* ctx, size_t batch, size_t heads, size_t head_dim, 
     return fail(UOCR_ERR_RESOURCE, "resource limit: host memory");
   }
   DeviceGuard g(ctx->device);
-  cudaError_t e = cudaMalloc(&kv->data, kv->bytes);
-  const size_t ints = batch * 2 + kvq_units(ctx->sms);
-  if (e == cudaSuccess) e = cudaMalloc(&kv->state, ints * sizeof(int));
-  if (e == cudaSuccess)
-    e = cudaMalloc(&kv->partial, kvq_units(ctx->sms) * (head_dim + 2) * sizeof(float));
-  if (e == cudaSuccess) e = cudaMemsetAsync(kv->data, 0, kv->bytes, ctx->stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(kv->state, 0, ints * sizeof(int), ctx->stream);
+  // one allocation: tiles (each a multiple of 256 bytes), counters and tickets, parts
+  const size_t units = kvq_units(ctx->sms), ints = batch * 2 + units;
+  const size_t all = kv->bytes + ints * sizeof(int) + units * (head_dim + 2) * sizeof(float);
+  cudaError_t e = cudaMalloc(&kv->data, all);
+  if (e == cudaSuccess) {
+    kv->state = reinterpret_cast<int*>(kv->data + kv->bytes);
+    kv->partial = reinterpret_cast<float*>(kv->state + ints);
+    e = cudaMemsetAsync(kv->data, 0, all, ctx->stream);
+  }
   if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
   if (e != cudaSuccess) {
     uocr_kvq_free(kv);
@@ -1927,8 +1929,6 @@ int uocr_kvq_free(uocr_kvq* kv) {
   if (!kv) return ok();
   DeviceGuard g(kv->device);
   if (kv->data) cudaFree(kv->data);
-  if (kv->state) cudaFree(kv->state);
-  if (kv->partial) cudaFree(kv->partial);
   delete kv;
   return ok();
 }

@@ -108,7 +108,7 @@ struct uocr_kvq {
   int batch = 0, width = 0, window = 0, max_prefix = 0;
   uocr::KvqLayout layout{};
   size_t bytes = 0;
-  unsigned char* data = nullptr;
+  unsigned char* data = nullptr;  // the tiles; state and partial lie behind them
   int* state = nullptr;     // [batch][2], then the attention's tickets
   float* partial = nullptr; // the attention's parts (KvqAttnArgs)
   std::vector<int> prefix;  // host mirror (0: not prefilled)
