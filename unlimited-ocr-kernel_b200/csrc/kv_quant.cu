@@ -9,6 +9,11 @@
 // with the differences and quotients in double, rounded half to even; the
 // cache stands for m + s * code.  m and s are rounded outwards so that the
 // codes reach every x: |x - (m + s code)| <= s / 2.
+//
+// Every kernel here may be resident while the kernel in front still writes what it
+// reads (programmatic dependent launches), so that nothing but a kernel's own
+// arguments is read-only for its whole life: loads are plain ones behind the wait,
+// never through the non-coherent path (no __ldg, no const __restrict__).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -115,7 +120,7 @@ __device__ __noinline__ uint32_t kvq_codes4_exactly(float x0, float x1, float x2
 template <bool VEC>
 __device__ __forceinline__ void kvq_load4(const float* row, int d, int dim, float (&x)[4]) {
   if (VEC) {
-    const float4 v = d < dim ? __ldg(reinterpret_cast<const float4*>(row + d))
+    const float4 v = d < dim ? *reinterpret_cast<const float4*>(row + d)
                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     x[0] = v.x;
     x[1] = v.y;
@@ -123,7 +128,7 @@ __device__ __forceinline__ void kvq_load4(const float* row, int d, int dim, floa
     x[3] = v.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = d + i < dim ? __ldg(row + d + i) : 0.0f;
+    for (int i = 0; i < 4; ++i) x[i] = d + i < dim ? row[d + i] : 0.0f;
   }
 }
 
@@ -161,8 +166,8 @@ void launch_kvq_reset(int* state, int seq, cudaStream_t st) {
 template <int BITS, bool VEC>
 __global__ void __launch_bounds__(256, 6)
     kvq_prefill_kernel(unsigned char* data, const KvqLayout L, int* state, int seq,
-                       const float* __restrict__ k, long long ld_k, const float* __restrict__ v,
-                       long long ld_v, int tokens, unsigned* status) {
+                       const float* k, long long ld_k, const float* v, long long ld_v, int tokens,
+                       unsigned* status) {
   extern __shared__ __align__(128) unsigned char kvq_stage[];
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
@@ -332,9 +337,8 @@ constexpr int kKvqPushWarps = 20;
 template <int BITS, bool ROPE>
 __global__ void __launch_bounds__(kKvqPushWarps * 32)
     kvq_push_kernel(unsigned char* data, const KvqLayout L, int* state, int window,
-                    const float* __restrict__ k, long long ld_k, const float* __restrict__ v,
-                    long long ld_v, float* q_out, const float2* __restrict__ table, int max_pos,
-                    unsigned* status) {
+                    const float* k, long long ld_k, const float* v, long long ld_v, float* q_out,
+                    const float2* table, int max_pos, unsigned* status) {
   constexpr int levels = (1 << BITS) - 1;
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
@@ -467,9 +471,8 @@ __device__ __forceinline__ int kvq_tokens(const int* state, int b, int window) {
 // and 69 us from 8 (6.2 and 6.3 TB/s; five CTAs per SM 62 and 71, eight 64 and 73).
 template <int BITS, bool VEC>
 __global__ void __launch_bounds__(256, 6)
-    kvq_read_kernel(const unsigned char* __restrict__ data, const KvqLayout L,
-                    const int* __restrict__ state, int window, int seq, long long first,
-                    long long count, float* k, float* v, unsigned* status) {
+    kvq_read_kernel(const unsigned char* data, const KvqLayout L, const int* state, int window, int seq,
+                    long long first, long long count, float* k, float* v, unsigned* status) {
   extern __shared__ __align__(128) unsigned char kvq_stage[];
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
@@ -477,8 +480,16 @@ __global__ void __launch_bounds__(256, 6)
   const long long tile = (first >> 5) + blockIdx.x / L.heads;
   const uint4* in = reinterpret_cast<const uint4*>(
       kvq_tile(const_cast<unsigned char*>(data), L, seq, h, tile * 32));
-  for (int i = threadIdx.x; i < L.tile / 16; i += 256)
-    reinterpret_cast<uint4*>(kvq_stage)[i] = __ldg(in + i);
+  // (three loads in flight per thread: an 8-bit tile of 128 dims in one round)
+  for (int i = threadIdx.x; i < L.tile / 16; i += 3 * 256) {
+    uint4 w[3];
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+      if (i + u * 256 < L.tile / 16) w[u] = in[i + u * 256];
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+      if (i + u * 256 < L.tile / 16) reinterpret_cast<uint4*>(kvq_stage)[i + u * 256] = w[u];
+  }
   const long long held = kvq_tokens(state, seq, window);
   const long long end = first + count < held ? first + count : held;
   if (held < first + count && blockIdx.x == 0 && threadIdx.x == 0) flag(status, DEV_KV_SLOT);
@@ -725,7 +736,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int d = grp * 32 + (i >> 2) * 16 + 4 * j + (i & 3);
-      const float qd = d < a.layout.dim ? __ldg(a.q + row + d) : 0.0f;
+      const float qd = d < a.layout.dim ? a.q[row + d] : 0.0f;
       v[i] = fmaf(qd, a.scale_rest, qd * a.scale);  // q log2(e) / sqrt(dim)
       big = fmaxf(big, fabsf(v[i]));
       sum += v[i];

@@ -245,7 +245,7 @@ __device__ __noinline__ void lp_join(LpShared& sh, const LpRow& row, int turns, 
 #pragma unroll
       for (int r = 0; r < kLpVec; ++r) {
         q[r] = r * 32 + lane < row.count(it, turns)
-                   ? __ldg(vec + row.start(it, turns) + r * 32 + lane)
+                   ? vec[row.start(it, turns) + r * 32 + lane]
                    : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       }
 #pragma unroll
@@ -259,7 +259,7 @@ __device__ __noinline__ void lp_join(LpShared& sh, const LpRow& row, int turns, 
     for (; hits; hits &= hits - 1) {
       const int e = row.index(it, turns, __ffs(hits) - 1);
       const int at = atomicAdd(&sh.count, 1);
-      if (at < kLpList) sh.list[at] = lp_key(__ldg(row.x + e), e);
+      if (at < kLpList) sh.list[at] = lp_key(row.x[e], e);
     }
   }
 }
@@ -277,7 +277,7 @@ __device__ __noinline__ void lp_pick_exactly(LpShared& sh, const LpRow& row, int
 #pragma unroll 4
     for (int i = 0; i < kLpPer; ++i) {
       const int e = first + i * kLpThreads + tid;
-      const float v = e < row.e1 ? __ldg(row.x + e) : 0.0f;
+      const float v = e < row.e1 ? row.x[e] : 0.0f;
       const LpKey key = e < row.e1 && !isnan(v) ? lp_key(v, e) : 0;
       best = key > best ? key : best;
     }
@@ -298,7 +298,7 @@ __device__ __noinline__ void lp_pick_exactly(LpShared& sh, const LpRow& row, int
       for (int i = 0; i < kLpPer; ++i) {
         const int e = first + i * kLpThreads + tid;
         if (e >= row.e1) break;
-        const float v = __ldg(row.x + e);
+        const float v = row.x[e];
         const LpKey key = isnan(v) ? 0 : lp_key(v, e);
         if (key != 0 && key >= floor) sh.list[atomicAdd(&sh.count, 1)] = key;
       }
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   float token_logit = 0.0f;
   if (a.tokens && rank == 0 && tid == 0) {
     token = a.tokens[row];
-    if (token >= 0 && token < a.vocab) token_logit = __ldg(part.x + token);
+    if (token >= 0 && token < a.vocab) token_logit = part.x[token];
   }
   if (tid == 0) {
     sh.count = 0;
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
             v[4 * r + 3] = q.w;
           }
       } else if (it >= turns && warp == 0 && lane < part.head + part.tail) {
-        v[0] = __ldg(part.x + part.index(it, turns, 0));
+        v[0] = part.x[part.index(it, turns, 0)];
       }
     }
     float mx = v[0];
