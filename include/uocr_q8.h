@@ -498,12 +498,16 @@ int uocr_kv_export(uocr_ctx *ctx, const uocr_kv *kv, size_t seq, float *keys_out
  *                      uocr_kv_rope_push_qkv (q_out apart from qkv);
  *   uocr_kvq_attention: softmax(q . K / sqrt(head_dim)) V of q row b over the
  *                      tokens of sequence b and what the cache stands for, FP32
- *                      accumulation (FP32 tolerance); a row of q that is not
+ *                      accumulation; a row of q that is not
  *                      finite (2^127 and above counts as such), or scores that are
  *                      not, give NaN outputs for that head and Numerical at the
- *                      next synchronising call (full
- *                      accuracy for 32 dims of q, and for steps of the values,
- *                      whose largest is 2^-86 and above); out may be q;
+ *                      next synchronising call; out may be q.  The 32 dims of a
+ *                      group share a fixed point: with R = (2^bits - 1) s, scores
+ *                      are within 2^-19 of sum |q| (|m| + R) / sqrt(head_dim), and
+ *                      outputs, beside what that moves the softmax's weights p by,
+ *                      within FP32 tolerance of sum p (|m| + R), where the largest
+ *                      |q| of a group and its largest p s are 2^-86 and above;
+ *                      weights below 2^-126 of the largest may count as 0;
  *   uocr_kvq_read:     what slots [first, first + count) of sequence seq stand
  *                      for, as token-major rows of floats (a head's slots lie in
  *                      the physical order of uocr_kv); slots past its tokens are

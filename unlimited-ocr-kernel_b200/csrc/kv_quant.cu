@@ -558,15 +558,16 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 //            from minus the running maximum: a score that counts ends near zero and
 //            costs no rounding of its own size;
 //   values:  rows = 16 dims, k = the tile's 32 tokens, columns = the four bytes
-//            of p_t s_t 2^a (< 2^31, a by the largest s so far);
+//            of p_t s_t 2^a (< 2^31, a by the largest p_t s_t of the group so far);
 //            o += 2^-a sum_b 256^b D_b, and p_t z_t is summed apart.
 //
 // Around the middle the sums stay near the size of what they stand for (from 0 up
 // they cancel against the least values, which cost a factor of two in accuracy).
 // Two neighbouring groups share an accumulator: a group's operand has its bytes
-// in its four columns and zeros in the other group's four.  Fixed point loses
-// less than a float does: 2^-31 of the group's largest |q|, 2^-30 of the largest
-// weight's size, against a float's 2^-24 of each term.
+// in its four columns and zeros in the other group's four.  The fixed points keep
+// 2^-31 of the group's largest |q| and 2^-31 to 2^-30 of its largest p_t s_t, so
+// that what they lose is below a float's rounding of the group's largest term; a
+// term that is 2^-7 of that one and less would have kept more in a float of its own.
 //
 // A tile is one bulk copy.  Every warp has a ring of its own, takes a run of
 // neighbouring tiles, and keeps its own maximum, sum and weighted values, so the
@@ -581,10 +582,8 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 // 32,768 tokens 15.4 us (7 us without its bytes).  The same from dequantised values
 // would need some 3 instructions an element, a scheduler's whole rate at this
 // bandwidth; here it is about 1.8 an element (ncu: 54 % of the issue slots).
-// Scores are in powers of two.  They may pass the running maximum by this much:
-// weights stay below 2^2.
-constexpr float kKvqSlack = 1.99f;
-constexpr int kKvqSlackBits = 2;
+// Scores are in powers of two.  They may pass the running maximum by this much.
+constexpr float kKvqSlack = 2.0f;
 // A tile whose scores lie further than this from the maximum that they were summed
 // against is summed again, unless a float at that maximum is too coarse for it.
 constexpr float kKvqFar = 8.0f, kKvqVast = 1048576.0f;
@@ -776,12 +775,13 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
 
   float m = 0.0f, l = 0.0f, middle[G], o[P][2][2];
   float start = 0.0f;  // of this lane's sums of scores: -m over the lanes of a row
-  int bound[G];  // largest step so far per group, as bf16 bits; -1 before the first turn
-  float wup[G], wdown[P];
+  // per group: the largest weight times step when the fixed point was last set, and
+  // what weights are scaled by and their sums scaled back
+  float seen[G], wup[G], wdown[P];
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     middle[i] = 0.0f;
-    bound[i] = -1;
+    seen[i] = 0.0f;
     wup[i] = 0.0f;
   }
 #pragma unroll
@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
     // ---- scores (of a tile past the warp's last: of whatever the slot holds, masked below)
     float score[N];  // against m
     uint32_t par[N][G];
-    bool in[N];
+    bool in[N] = {};
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const unsigned char* kt = tile + u * kTileBytes;
@@ -851,29 +851,39 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
       const float r1 = (j & 2 ? x[3] : x[1]) + __shfl_xor_sync(0xffffffffu, j & 2 ? x[1] : x[3], 2);
       score[u] = (j & 1 ? r1 : r0) + __shfl_xor_sync(0xffffffffu, j & 1 ? r0 : r1, 1);
     }
-    // ---- the steps and least values of the tokens that are there
-    bool over = false;
+    // ---- the steps and least values of the tokens that are there, and the weights' bytes
+    // as they are where neither the maximum nor the fixed point has to move
+    float pr[N];
+    bool over = it == first;
+    auto weigh = [&](int u) {
+      pr[u] = in[u] ? exp2_fast(score[u]) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const float w = pr[u] * bf16_low(par[u][i]) * wup[i];
+        over |= w >= 2147483648.0f;
+        sh.weights[warp][u][i][t] = __float2uint_rn(w);
+      }
+    };
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       in[u] = (it + u) * 32 + t < end;
       over |= in[u] && score[u] > kKvqSlack;
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
+      for (int i = 0; i < G; ++i)
         par[u][i] = in[u] ? *reinterpret_cast<const uint32_t*>(tile + u * kTileBytes + kTileBytes / 2 +
                                                                kCodes + i * 128 + lane * 4)
                           : 0;
-        over |= static_cast<int>(par[u][i] & 0xFFFFu) > bound[i];
-      }
+      weigh(u);
     }
     // ---- softmax: m, the maximum that scores and weights refer to, is raised only
-    // when a score passes it by kKvqSlack, the bounds only when a step passes them:
-    // one vote for all in most turns
+    // when a score passes it by kKvqSlack, the fixed points only when a weight times
+    // its step passes them: one vote for all in most turns
     if (__any_sync(0xffffffffu, over)) {
       float top = -INFINITY;
 #pragma unroll
       for (int u = 0; u < N; ++u) top = fmaxf(top, in[u] ? score[u] : -INFINITY);
       top = warp_max(top);
-      float raise = 0.0f;
+      float raise = 0.0f, keep = 1.0f;
       if (top > 0.0f || it == first) {
         const float old = m;
         m = old + top;
@@ -881,7 +891,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
         // so that it weighs 1 whatever m was rounded to)
         raise = fabsf(m) < kKvqVast ? m - old : top;
         start = j & 1 ? -0.5f * m : 0.0f;
-        const float keep = it == first ? 0.0f : exp2_fast(-raise);
+        keep = it == first ? 0.0f : exp2_fast(-raise);
         l *= keep;
 #pragma unroll
         for (int i = 0; i < G; ++i) middle[i] *= keep;
@@ -893,40 +903,44 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
           o[p][1][1] *= keep;
         }
       }
+      // the fixed point of a group: its largest weight times step so far, as it stands
+      // to m, lies in its upper half.  (By the largest step alone, a token of no weight
+      // whose values are 10^5 times the others' would cost them their bits.)
+      int e[G];
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        score[u] -= raise;
+        pr[u] = in[u] ? exp2_fast(score[u]) : 0.0f;
+      }
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        uint32_t big = 0;
+        float big = 0.0f;
 #pragma unroll
-        for (int u = 0; u < N; ++u) big = max(big, par[u][i] & 0xFFFFu);
-        bound[i] = max(bound[i], static_cast<int>(__reduce_max_sync(0xffffffffu, big)));
-        // step < 2^(e - 126), weight < 2^2; steps below 2^-86 lose precision
-        const int e = max(bound[i] >> 7, 40);
-        wup[i] = __uint_as_float(static_cast<uint32_t>(284 - kKvqSlackBits - e) << 23);
+        for (int u = 0; u < N; ++u) big = fmaxf(big, pr[u] * bf16_low(par[u][i]));  // (NaN counts as nothing)
+        seen[i] = fmaxf(seen[i] * keep, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
+        // weight times step < 2^(e - 126); below 2^-86 they lose precision
+        e[i] = max(static_cast<int>(__float_as_uint(seen[i]) >> 23), 40);
+        wup[i] = __uint_as_float(static_cast<uint32_t>(284 - e[i]) << 23);
       }
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        const int bd = acc_group && 2 * p + 1 < G ? bound[min(2 * p + 1, G - 1)] : bound[2 * p];
-        wdown[p] = __uint_as_float(static_cast<uint32_t>(max(bd >> 7, 40) - 30 - kShift + kKvqSlackBits + (j & 1) * 16) << 23);
+        const int ep = acc_group && 2 * p + 1 < G ? e[min(2 * p + 1, G - 1)] : e[2 * p];
+        wdown[p] = __uint_as_float(static_cast<uint32_t>(ep - 30 - kShift + (j & 1) * 16) << 23);
       }
       if (fabsf(raise) > kKvqFar && fabsf(m) < kKvqVast && !again) {
         again = true;
         continue;
       }
 #pragma unroll
-      for (int u = 0; u < N; ++u) score[u] -= raise;
+      for (int u = 0; u < N; ++u) weigh(u);
     }
     again = false;
-    // ---- the weights' bytes
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const float pr = in[u] ? exp2_fast(score[u]) : 0.0f;
-      l += pr;
+      l += pr[u];
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const float step = bf16_low(par[u][i]);
-        middle[i] = fmaf(pr, fmaf(kMiddle, step, bf16_high(par[u][i])), middle[i]);
-        sh.weights[warp][u][i][t] = __float2uint_rn(pr * (step * wup[i]));
-      }
+      for (int i = 0; i < G; ++i)
+        middle[i] = fmaf(pr[u], fmaf(kMiddle, bf16_low(par[u][i]), bf16_high(par[u][i])), middle[i]);
     }
     __syncwarp();
     // ---- values
