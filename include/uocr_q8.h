@@ -498,10 +498,12 @@ int uocr_kv_export(uocr_ctx *ctx, const uocr_kv *kv, size_t seq, float *keys_out
  *                      uocr_kv_rope_push_qkv (q_out apart from qkv);
  *   uocr_kvq_attention: softmax(q . K / sqrt(head_dim)) V of q row b over the
  *                      tokens of sequence b and what the cache stands for, FP32
- *                      accumulation; a row of q that is not
- *                      finite (2^127 and above counts as such), or scores that are
- *                      not, give NaN outputs for that head and Numerical at the
- *                      next synchronising call; out may be q.  The 32 dims of a
+ *                      accumulation; out may be q.  A row of q that is not
+ *                      finite (2^127 and above counts as such), or scores whose
+ *                      sums in FP32 are not, give NaN outputs for that head and
+ *                      Numerical at the next synchronising call, but for scores
+ *                      that fall to -inf: they weigh nothing, unless a head has no
+ *                      other (NaN and Numerical).  The 32 dims of a
  *                      group share a fixed point: with R = (2^bits - 1) s, scores
  *                      are within 2^-19 of sum |q| (|m| + R) / sqrt(head_dim), and
  *                      outputs, beside what that moves the softmax's weights p by,

@@ -159,3 +159,58 @@ def test_outlying_channels_of_the_query(ctx, bits, size):
     move = np.expm1(2 * off.max(-1, keepdims=True)) + EPS * (100 + 3 * np.sqrt(tokens))
     assert np.all(np.abs(out - ref) <= move * terms), np.max(np.abs(out - ref) / (move * terms))
     kv.free()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("where", ["one", "first tiles", "last tiles", "all but one", "all but a pushed one"])
+def test_scores_below_the_least_float(ctx, bits, where):
+    """Scores of -inf weigh nothing, wherever they lie: as if their tokens were not there."""
+    rng = np.random.default_rng(len(where) + bits)
+    heads, dim, tokens, pushes = 3, 64, 400, 2
+    low = np.zeros(tokens + pushes, bool)
+    low[{"one": slice(7, 8), "first tiles": slice(0, 200), "last tiles": slice(100, tokens + pushes),
+         "all but one": slice(0, tokens + pushes), "all but a pushed one": slice(0, tokens + pushes)}[where]] = True
+    if where.startswith("all"):
+        low[tokens + 1 if "pushed" in where else 333] = False
+    big = np.float32(2.0 ** 30)
+    q = np.full((heads, dim), big)
+    k, v = (rng.standard_normal((tokens + pushes, heads, dim)).astype(np.float32) for _ in range(2))
+    k /= 4 * big
+    k[low, 1:] = -np.float32(2.0 ** 99)  # (the first head has no such score)
+    rows = [x.reshape(tokens + pushes, -1) for x in (k, v)]
+    for batch in (1, 260):  # a head spread over clusters, and one CTA per head
+        kv = QuantizedKvCache(ctx, batch, heads, dim, pushes, tokens, bits)
+        for b in range(batch):
+            kv.prefill(b, dev(rows[0][:tokens]), dev(rows[1][:tokens]))
+        for i in range(tokens, tokens + pushes):
+            kv.push(*(dev(np.repeat(x[i:i + 1], batch, 0)) for x in rows))
+        out = host(kv.attention(dev(np.repeat(q.reshape(1, -1), batch, 0)))).reshape(batch, heads, dim)
+        ctx.sync()
+        for h, there in ((0, np.ones_like(low)), (1, ~low), (2, ~low)):
+            parts = ([t[:, None] for t in map(lambda t: t[there, h], held(x, bits))] for x in (k, v))
+            ref, tol = reference(q[h:h + 1], *parts)
+            assert np.all(np.abs(out[-1, h] - ref[0]) <= tol[0]), (h, np.max(np.abs(out[-1, h] - ref[0]) / tol[0]))
+        kv.free()
+
+
+@pytest.mark.parametrize("sign,where", [(1.0, "one"), (1.0, "first tiles"), (1.0, "last"), (1.0, "all"), (-1.0, "all")])
+def test_scores_that_are_not_finite(ctx, sign, where):
+    """One score of +inf, or nothing but -inf: NaN for that head alone, and Numerical."""
+    rng = np.random.default_rng(len(where))
+    heads, dim, tokens = 3, 64, 400
+    low = {"one": slice(7, 8), "first tiles": slice(0, 70), "last": slice(399, 400), "all": slice(0, 400)}[where]
+    q = np.full((1, heads * dim), np.float32(2.0 ** 30))
+    k, v = (rng.standard_normal((tokens, heads, dim)).astype(np.float32) for _ in range(2))
+    k *= np.float32(2.0 ** -32)
+    k[low, 1] = np.float32(sign * 2.0 ** 99)
+    for batch in (1, 260):
+        kv = QuantizedKvCache(ctx, batch, heads, dim, 1, tokens, 4)
+        for b in range(batch):
+            kv.prefill(b, dev(k.reshape(tokens, -1)), dev(v.reshape(tokens, -1)))
+        out = host(kv.attention(dev(np.repeat(q, batch, 0)))).reshape(batch, heads, dim)
+        import uocr_q8
+        with pytest.raises(uocr_q8.OcrError) as e:
+            ctx.sync()
+        assert e.value.kind == "Numerical"
+        assert np.all(np.isnan(out[:, 1])) and np.all(np.isfinite(out[:, ::2]))
+        kv.free()

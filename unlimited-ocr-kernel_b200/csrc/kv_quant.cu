@@ -792,6 +792,9 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
 
   const int t = g + 8 * j;  // the token of a tile that this lane weighs
   bool again = false;  // this turn's scores are summed a second time
+  // no score but -inf so far: m is none of them.  A score of -inf (below the least
+  // float) weighs nothing, in this warp or another; a head with no other has no sum
+  bool fresh = true;
   for (int it = first, slot = 0, phase = 0; it < last;) {
     if (!__all_sync(0xffffffffu, mbar_wait_try(&sh.full[warp][slot], phase, a.status))) {
       // (a safety net: flagged) copies in flight land before the CTA ends
@@ -854,7 +857,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
     // ---- the steps and least values of the tokens that are there, and the weights' bytes
     // as they are where neither the maximum nor the fixed point has to move
     float pr[N];
-    bool over = it == first;
+    bool over = fresh;
     auto weigh = [&](int u) {
       pr[u] = in[u] ? exp2_fast(score[u]) : 0.0f;
 #pragma unroll
@@ -884,14 +887,15 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
       for (int u = 0; u < N; ++u) top = fmaxf(top, in[u] ? score[u] : -INFINITY);
       top = warp_max(top);
       float raise = 0.0f, keep = 1.0f;
-      if (top > 0.0f || it == first) {
+      if (top > 0.0f || (fresh && top > -INFINITY)) {
         const float old = m;
         m = old + top;
         // (2^20 and above, where a place of m is 1/8 and more: against this tile's top,
         // so that it weighs 1 whatever m was rounded to)
         raise = fabsf(m) < kKvqVast ? m - old : top;
         start = j & 1 ? -0.5f * m : 0.0f;
-        keep = it == first ? 0.0f : exp2_fast(-raise);
+        keep = fresh ? 0.0f : exp2_fast(-raise);
+        fresh = false;
         l *= keep;
 #pragma unroll
         for (int i = 0; i < G; ++i) middle[i] *= keep;
@@ -1011,7 +1015,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
           sh.o[warp][(2 * p + acc_group) * 32 + mb * 16 + up * 8 + g] = v + add;
       }
   if (lane == 0) {
-    sh.m[warp] = first < last ? m : -INFINITY;
+    sh.m[warp] = fresh ? -INFINITY : m;
     sh.l[warp] = l;
   }
   __syncthreads();
