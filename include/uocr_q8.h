@@ -93,8 +93,9 @@ int uocr_ctx_sync(uocr_ctx *ctx);
 int uocr_ctx_device(const uocr_ctx *ctx, int *device, int *sm_count);
 /* No counterpart in the reference (which has no device waits).  The bounded
  * device waits of the context's kernels (the one-token decode kernel's grid
- * barrier) give up after `ns` nanoseconds (0: the default, about 2 s) and
- * report UOCR_ERR_TIMEOUT at the next synchronising call. */
+ * barrier; the bulk copies of uocr_kvq_attention and uocr_token_logprobs) give
+ * up after `ns` nanoseconds (0: the default, about 2 s) and report
+ * UOCR_ERR_TIMEOUT at the next synchronising call. */
 int uocr_ctx_set_wait_limit(uocr_ctx *ctx, uint64_t ns);
 /* Failure-detection test hook, host-side (no GPU fault): while `hold` is
  * nonzero, the one-token decode kernel's grid barrier waits for one arrival
@@ -102,6 +103,10 @@ int uocr_ctx_set_wait_limit(uocr_ctx *ctx, uint64_t ns);
  * the next synchronising call reports UOCR_ERR_TIMEOUT.  The barrier's words
  * stay valid: after the hold is cleared the next launch is exact again. */
 int uocr_ctx_hold_decode_barrier(uocr_ctx *ctx, int hold);
+/* The same for the bulk copies of uocr_kvq_attention and uocr_token_logprobs:
+ * while `hold` is nonzero every wait for one runs out its limit.  The launch
+ * returns, its outputs are NaN (ids -1), and the next one is exact again. */
+int uocr_ctx_hold_copies(uocr_ctx *ctx, int hold);
 
 /* ---- matrices: Int8Matrix (src/cpu/quantized.rs:11-237) -----------------
  * Int8Matrix::from_parts (:18-42): copies host weights/scales to the device.

@@ -303,6 +303,12 @@ int uocr_ctx_hold_decode_barrier(uocr_ctx* ctx, int hold) {
   return ok();
 }
 
+int uocr_ctx_hold_copies(uocr_ctx* ctx, int hold) {
+  if (!ctx) return fail(UOCR_ERR_INVALID, "null context");
+  ctx->hold_copies = hold ? 1 : 0;
+  return ok();
+}
+
 int uocr_ctx_device(const uocr_ctx* ctx, int* device, int* sm_count) {
   if (!ctx) return fail(UOCR_ERR_INVALID, "null context");
   if (device) *device = ctx->device;
@@ -1862,6 +1868,13 @@ int uocr_kv_export(uocr_ctx* ctx, const uocr_kv* kv, size_t seq, float* keys_out
   return check_launch();
 }
 
+// Waits of the kernels below for their bulk copies (cycles as for the decode
+// barrier: at the maximum clock, rounded up).
+static BulkWait bulk_wait(const uocr_ctx* ctx) {
+  return {ctx->wait_ns ? static_cast<long long>(ctx->wait_ns * 2) : kWaitLimitCycles,
+          ctx->hold_copies ? 1u : 0u};
+}
+
 // ---- KV cache held in 4 or 8 bits ---------------------------------------------
 // The states and rules of uocr_kv (LayerCache, src/decoder/cache.rs:3-95) over
 // quantised storage; no counterpart in the reference.
@@ -2054,6 +2067,7 @@ int uocr_kvq_attention(uocr_ctx* ctx, const uocr_kvq* kv, const float* q_dev, fl
   a.sms = ctx->sms;
   a.partial = kv->partial;
   a.tickets = kv->state + 2 * kv->batch;
+  a.wait = bulk_wait(ctx);
   const cudaError_t e = launch_kvq_attention(a, kv->batch, ctx->stream);
   if (e != cudaSuccess) return fail(UOCR_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
   return ok();
@@ -2121,6 +2135,7 @@ int uocr_token_logprobs(uocr_ctx* ctx, const float* logits_dev, size_t rows, siz
   a.top_ids = reinterpret_cast<long long*>(top_ids_dev);
   a.top_logprobs = top_logprobs_dev;
   a.status = ctx->status_dev;
+  a.wait = bulk_wait(ctx);
   const cudaError_t e = launch_token_logprobs(a, static_cast<int>(rows), ctx->sms, ctx->stream);
   if (e != cudaSuccess) return fail(UOCR_ERR_CUDA, "log probabilities launch: %s", cudaGetErrorString(e));
   return ok();

@@ -372,11 +372,12 @@ __device__ __forceinline__ bool mbar_wait_spin(uint64_t* bar, uint32_t parity, u
 // the hardware may suspend the thread until the phase completes, so warps
 // that wait leave their issue slots to the warps doing the work (a test_wait
 // spin by many warps starves the workers of the same scheduler).
-__device__ __forceinline__ bool mbar_wait_try(uint64_t* bar, uint32_t parity, unsigned* status) {
+__device__ __forceinline__ bool mbar_wait_try(uint64_t* bar, uint32_t parity, unsigned* status,
+                                              long long limit_cycles = kWaitLimitCycles) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try_wait(bar, parity)) {
-    if (clock64() - t0 > kWaitLimitCycles) {
+    if (clock64() - t0 > limit_cycles) {
       flag(status, DEV_TIMEOUT);
       return false;
     }

@@ -48,6 +48,7 @@ struct uocr_ctx {
   // uocr_ctx_set_wait_limit (0: the kernels' default) and the failure-detection
   // test hook uocr_ctx_hold_decode_barrier
   uint64_t wait_ns = 0;
+  int hold_copies = 0;
   int hold_barrier = 0;
 };
 

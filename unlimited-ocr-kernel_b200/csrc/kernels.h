@@ -362,6 +362,13 @@ void launch_kvq_rope_push(unsigned char* data, const KvqLayout& L, int* state, i
 void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* state, int window,
                      int seq, long long first, long long count, float* k, float* v, unsigned* status,
                      cudaStream_t st);
+// Bounded waits for bulk copies: SM cycles after which one gives up, and arrivals
+// that never come (failure-detection hook).
+struct BulkWait {
+  long long cycles;
+  unsigned extra;
+};
+
 struct KvqAttnArgs {
   const unsigned char* data;
   KvqLayout layout;
@@ -377,6 +384,7 @@ struct KvqAttnArgs {
   float* partial;
   int* tickets;
   int splits, parts;  // CTAs per cluster, clusters per head: set by the launcher
+  BulkWait wait;
 };
 constexpr int kKvqMaxParts = 16;
 // Heads are spread over several clusters (of two CTAs at least) only while
@@ -399,6 +407,7 @@ struct LogprobArgs {
   float* top_logprobs;       // the same
   unsigned* status;
   int splits;                // CTAs per row: set by the launcher
+  BulkWait wait;
 };
 constexpr int kLogprobMaxTop = 32;
 cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t st);

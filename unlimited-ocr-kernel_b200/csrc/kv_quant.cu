@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
              &sh.full[warp][slot]);
   };
   if (lane == 0) {
-    for (int i = 0; i < kKvqSlots; ++i) mbar_init(&sh.full[warp][i], 1);
+    for (int i = 0; i < kKvqSlots; ++i) mbar_init(&sh.full[warp][i], 1 + a.wait.extra);
     fence_mbar_init();
     for (int i = 0; i < kKvqSlots && first + i * N < last; ++i) fetch(first + i * N, i);
   }
@@ -796,15 +796,16 @@ __global__ void __launch_bounds__(kvq_warps(G, BITS) * 32) kvq_attention_kernel(
   // float) weighs nothing, in this warp or another; a head with no other has no sum
   bool fresh = true;
   for (int it = first, slot = 0, phase = 0; it < last;) {
-    if (!__all_sync(0xffffffffu, mbar_wait_try(&sh.full[warp][slot], phase, a.status))) {
-      // (a safety net: flagged) copies in flight land before the CTA ends
+    if (!__all_sync(0xffffffffu, mbar_wait_try(&sh.full[warp][slot], phase, a.status, a.wait.cycles))) {
+      // (a safety net: flagged, the head is NaN) copies in flight land before the CTA ends
       for (int i = 1; i < kKvqSlots && it + i * N < last; ++i) {
         if (++slot == kKvqSlots) {
           slot = 0;
           phase ^= 1;
         }
-        mbar_wait_try(&sh.full[warp][slot], phase, a.status);
+        mbar_wait_try(&sh.full[warp][slot], phase, a.status, a.wait.cycles);
       }
+      l = __uint_as_float(0x7FC00000u);
       break;
     }
     const unsigned char* tile = sh.ring[warp][slot];

@@ -99,6 +99,7 @@ struct LpShared {
   uint32_t bound[2 * kLogprobMaxTop + kLpWarps];
   int count;                                 // candidates that have joined
   int over;                                  // more than the list holds
+  int lost;                                  // a copy has not landed in time
 };
 
 // The k best of the list's n, in order, into sh.best; the k-th best, where there
@@ -311,6 +312,16 @@ __device__ __noinline__ void lp_pick_exactly(LpShared& sh, const LpRow& row, int
   __syncthreads();
 }
 
+// The copies of the warp's turns from `it` on have not landed in time (a safety net:
+// flagged): those in flight, before turn `end`, are waited for again, so that none
+// lands behind the CTA's end.
+__device__ __noinline__ void lp_give_up(LpShared& sh, int it, int end, unsigned* status, long long cycles) {
+#pragma unroll 1
+  for (int i = it; i < it + kLpStages && i < end; ++i)
+    mbar_wait_try(&sh.full[threadIdx.x >> 5][i % kLpStages], i / kLpStages & 1, status, cycles);
+  sh.lost = 1;  // (read behind barriers)
+}
+
 template <bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LogprobArgs a) {
   extern __shared__ __align__(128) unsigned char lp_raw[];
@@ -346,7 +357,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
              &sh.full[warp][slot]);
   };
   if (lane == 0) {
-    for (int i = 0; i < kLpStages; ++i) mbar_init(&sh.full[warp][i], 1);
+    for (int i = 0; i < kLpStages; ++i) mbar_init(&sh.full[warp][i], 1 + a.wait.extra);
     fence_mbar_init();
     for (int i = 0; i < kLpStages && i < turns; ++i) fetch(i, i);
   }
@@ -359,6 +370,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   if (tid == 0) {
     sh.count = 0;
     sh.over = 0;
+    sh.lost = 0;
     sh.floor = 0;
   }
   __syncthreads();
@@ -368,6 +380,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   float2 s2 = make_float2(0.0f, 0.0f), w2 = make_float2(0.0f, 0.0f);
   float best = -INFINITY;  // of this lane, since turn `from`
   int from = 0;
+  int stop = turns;  // where a wait gives up: its turn; no more copies are waited for or started
   // the candidates of turns [from, to)
   auto gather = [&](int to) {
     lp_bound(sh, lp_order(best), k);
@@ -377,9 +390,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
 #pragma unroll 1
   for (int it = 0, slot = 0, phase = 0; it < all_turns; ++it) {
     float v[kLpPer];
-    const int here = it < turns ? part.count(it, turns) : 0;
+    const int here = it < stop ? part.count(it, turns) : 0;
     if (here == kLpTurn) {
-      mbar_wait_try(&sh.full[warp][slot], phase, a.status);
+      if (!mbar_wait_try(&sh.full[warp][slot], phase, a.status, a.wait.cycles)) stop = it;
 #pragma unroll
       for (int r = 0; r < kLpVec; ++r) {
         const float4 q = sh.ring[warp][slot][r * 32 + lane];
@@ -392,7 +405,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
 #pragma unroll
       for (int i = 0; i < kLpPer; ++i) v[i] = -INFINITY;
       if (here > 0) {
-        mbar_wait_try(&sh.full[warp][slot], phase, a.status);
+        if (!mbar_wait_try(&sh.full[warp][slot], phase, a.status, a.wait.cycles)) stop = it;
 #pragma unroll
         for (int r = 0; r < kLpVec; ++r)
           if (r * 32 + lane < here) {
@@ -415,7 +428,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
       sh.kept[it - from][tid] = lp_up16(mx);
     }
     __syncwarp();  // every lane has read the slot
-    if (lane == 0 && it + kLpStages < turns) fetch(it + kLpStages, slot);
+    if (lane == 0 && it + kLpStages < stop) fetch(it + kLpStages, slot);
     if (++slot == kLpStages) {
       slot = 0;
       phase ^= 1;
@@ -467,6 +480,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     }
   }
   float s = s2.x + s2.y, w = w2.x + w2.y;
+  if (stop < turns) {
+    lp_give_up(sh, stop, part.count(turns - 1, turns) ? turns : turns - 1, a.status, a.wait.cycles);
+    s = __uint_as_float(0x7FC00000u);  // (the row is NaN)
+  }
   if (TOP && all_turns) gather(all_turns);
 
   // ---- the CTA's sums, and its k best in order
@@ -486,9 +503,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   }
   int held = 0;
   if (TOP) {  // (every join lies behind the barrier above)
-    held = sh.count;
+    const bool gone = sh.lost;  // (the row is NaN, and the ring may still be written)
+    held = gone ? 0 : sh.count;
     // the list has run full, or k logits that are not -inf have not been found
-    if (sh.over || held > kLpList || (held < k && held < part.e1 - part.e0)) {
+    if (!gone && (sh.over || held > kLpList || (held < k && held < part.e1 - part.e0))) {
       __syncthreads();
       lp_pick_exactly(sh, part, k);
       held = sh.count;

@@ -115,6 +115,12 @@ class GpuContext:
         barrier waits for an arrival that never comes until released."""
         _check(lib().uocr_ctx_hold_decode_barrier(self._h, int(bool(hold))))
 
+    def hold_copies(self, hold: bool) -> None:
+        """Failure-detection test hook: the attention over a quantised cache and
+        the token log probabilities wait for bulk copies that never arrive until
+        released."""
+        _check(lib().uocr_ctx_hold_copies(self._h, int(bool(hold))))
+
     def sm_count(self) -> int:
         d, s = ctypes.c_int(), ctypes.c_int()
         _check(lib().uocr_ctx_device(self._h, ctypes.byref(d), ctypes.byref(s)))
