@@ -554,9 +554,10 @@ int uocr_kvq_read(uocr_ctx *ctx, const uocr_kvq *kv, size_t seq, size_t first, s
  *                 (top_k <= 32 and <= vocab; 0: none; vocab <= 2^30).
  * -inf is a logit of probability 0 (a banned token).  A row that holds NaN or
  * +inf, or nothing but -inf, gives NaN (ids -1) and Numerical at the next
- * synchronising call; a token id of vocab or above NaN and Shape.  Sums in FP32,
- * the maximum's own term kept apart, so that a nearly certain token's log
- * probability and a nearly zero entropy keep an FP32 relative precision.
+ * synchronising call; a token id of vocab or above NaN and Shape.  Sums in FP32
+ * over at most 512 terms one after the other (in 64 bits above them), the
+ * maximum's own term kept apart, so that a nearly certain token's log probability
+ * and a nearly zero entropy keep an FP32 relative precision.
  * Asynchronous on the context's stream; allocates nothing. */
 int uocr_token_logprobs(uocr_ctx *ctx, const float *logits_dev, size_t rows, size_t vocab, size_t ld,
                         const int64_t *tokens_dev, size_t top_k, float *logprob_dev,

@@ -46,6 +46,11 @@ constexpr int kLpTurn = 32 * kLpVec;         // vectors per warp and turn: one b
 constexpr int kLpStages = 2;
 constexpr int kLpCluster = 8;                // most CTAs per row (portable)
 constexpr int kLpKept = 32;                  // turns whose maxima are kept
+// Terms are summed in FP32, eight of a turn to an accumulator.  Where a warp takes more
+// than kLpSerialTurns, they join sums in 64 bits every kLpSerial turns: 512 equal terms
+// one after the other are off by 256 steps of 2^-24 at most, but the 262,144 of a flat
+// row of 2^30 by 0.4 %.  (In every kernel 0.6 us of 5.2 for one row, 2 % for 1,517.)
+constexpr int kLpSerialTurns = 64, kLpSerial = 16;
 // Candidates: at most kLpCut stay after a cut, kLogprobMaxTop threads' elements
 // join by the exact bound.
 constexpr int kLpList = 768;
@@ -156,6 +161,13 @@ __device__ __forceinline__ void lp_refer(float m, float M, float& s, float& w, f
   w = f * fmaf(d, all, w);
   s = f * all;
   n = 0.0f;
+}
+
+// The same for sums in 64 bits, of which none equals the old maximum.
+__device__ __noinline__ double2 lp_refer_far(float m, float M, double2 sw) {
+  const float d = fmaxf(m - M, -1000.0f);
+  const double f = lp_exp2(d * kLpLog2e);
+  return make_double2(f * sw.x, f * (sw.y + d * sw.x));
 }
 
 __device__ __forceinline__ float lp_max3(float a, float b, float c) {
@@ -322,7 +334,8 @@ __device__ __noinline__ void lp_give_up(LpShared& sh, int it, int end, unsigned*
   sh.lost = 1;  // (read behind barriers)
 }
 
-template <bool TOP>
+// TOP: alternatives; LONG: rows of many turns.
+template <bool TOP, bool LONG>
 __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LogprobArgs a) {
   extern __shared__ __align__(128) unsigned char lp_raw[];
   LpShared& sh = *reinterpret_cast<LpShared*>(lp_raw);
@@ -377,6 +390,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
   // The warp's maximum so far, and sums that refer to it and leave one instance of
   // it out, in the lane whose n is 1.
   float m = -INFINITY, n = 0.0f;
+  double2 far = make_double2(0.0, 0.0);  // both, of the turns that are no longer in s2, w2
   float2 s2 = make_float2(0.0f, 0.0f), w2 = make_float2(0.0f, 0.0f);
   float best = -INFINITY;  // of this lane, since turn `from`
   int from = 0;
@@ -441,6 +455,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
       lp_refer(m, top, s, w, n);
       s2 = make_float2(s, 0.0f);
       w2 = make_float2(w, 0.0f);
+      if (LONG && it >= kLpSerial) far = lp_refer_far(m, top, far);
       m = top;
       const unsigned who = __ballot_sync(0xffffffffu, mx == m);
       if (lane == __ffs(who) - 1) {
@@ -465,6 +480,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
       s2 = f2_add(s2, e);
       w2 = f2_fma(e, z, w2);
     }
+    if (LONG && it % kLpSerial == kLpSerial - 1) {
+      far.x += s2.x + s2.y;
+      far.y += w2.x + w2.y;
+      s2 = w2 = make_float2(0.0f, 0.0f);
+    }
     if (TOP && it + 1 - from == kLpKept && it + 1 < all_turns) {
       gather(it + 1);
       const int held = sh.count;  // (written next behind a barrier)
@@ -480,6 +500,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     }
   }
   float s = s2.x + s2.y, w = w2.x + w2.y;
+  if (LONG) {
+    s = static_cast<float>(far.x + s);
+    w = static_cast<float>(far.y + w);
+  }
   if (stop < turns) {
     lp_give_up(sh, stop, part.count(turns - 1, turns) ? turns : turns - 1, a.status, a.wait.cycles);
     s = __uint_as_float(0x7FC00000u);  // (the row is NaN)
@@ -608,7 +632,7 @@ static int lp_clusters(int splits, int per, cudaLaunchConfig_t cfg) {
   int n = 0;
   cfg.gridDim = dim3(splits);
   cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, token_logprobs_kernel<true>, &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, token_logprobs_kernel<true, false>, &cfg) != cudaSuccess) {
     cudaGetLastError();
     n = 0;
   }
@@ -622,10 +646,9 @@ cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t
   static_assert(4 * (smem + 1024) <= kLpSmemSm, "four CTAs per SM");
   static PerDeviceOnce configured;
   configured.run([] {
-    cudaFuncSetAttribute(token_logprobs_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         kLpSmemSm / 2 - 1024);
-    cudaFuncSetAttribute(token_logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         kLpSmemSm / 2 - 1024);
+    for (auto kernel : {token_logprobs_kernel<true, false>, token_logprobs_kernel<true, true>,
+                        token_logprobs_kernel<false, false>, token_logprobs_kernel<false, true>})
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLpSmemSm / 2 - 1024);
   });
   // CTAs per row: while three per SM hold them all and each has a full ring (64
   // rows of 129,280 logits with five alternatives: 15.2 us by 4, 16.4 by 8, 19.3 by
@@ -634,6 +657,7 @@ cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t
   while (a.splits < kLpCluster && 2LL * rows * a.splits <= 3LL * sms &&
          a.vocab > 4LL * kLpTurn * kLpWarps * a.splits)
     a.splits *= 2;
+  const bool far = a.vocab > static_cast<long long>(kLpSerialTurns) * kLpTurn * 4 * kLpWarps * a.splits;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {static_cast<unsigned>(a.splits), 1, 1};
@@ -659,7 +683,9 @@ cudaError_t launch_token_logprobs(LogprobArgs a, int rows, int sms, cudaStream_t
   for (int done = 0; done < rows; done += kMost) {
     const int now = rows - done < kMost ? rows - done : kMost;
     cfg.gridDim = dim3(static_cast<unsigned>(now) * a.splits);
-    auto kernel = a.top_k ? token_logprobs_kernel<true> : token_logprobs_kernel<false>;
+    auto kernel = a.top_k ? far ? token_logprobs_kernel<true, true> : token_logprobs_kernel<true, false>
+                  : far   ? token_logprobs_kernel<false, true>
+                          : token_logprobs_kernel<false, false>;
     cfg.numAttrs = 2;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
     if (e != cudaSuccess) {  // without the early start
