@@ -225,6 +225,7 @@ class QuantizedKvCache:
         self.ctx = ctx
         self.batch, self.heads, self.head_dim, self.bits = batch, heads, head_dim, bits
         self.width = heads * head_dim
+        self._slots = max_prefix + window
         h = ctypes.c_void_p()
         self._lib = lib()
         _check(self._lib.uocr_kvq_create(ctx.handle, batch, heads, head_dim, window, max_prefix,
@@ -296,6 +297,9 @@ class QuantizedKvCache:
     def read(self, seq: int, first: int, count: int, keys_t=None, values_t=None):
         """What slots [first, first + count) of sequence seq stand for:
         token-major rows [count x width] of keys and of values."""
+        if not 0 <= count <= self._slots:  # (before rows of that many are allocated)
+            from . import OcrError
+            raise OcrError(4, "invalid tensor shape: slots past the tokens of the cache")
         if keys_t is None:
             keys_t = self._new(count)
         else:

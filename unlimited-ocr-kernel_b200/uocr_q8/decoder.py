@@ -347,11 +347,12 @@ def token_logprobs_device(ctx: GpuContext, logits_t, tokens_t=None, top_k: int =
     if top_k < 0:
         from . import OcrError
         raise OcrError(4, "invalid tensor shape: top_k must not be negative")
+    room = top_k if top_k <= 32 else 0  # (more are refused by the call: nothing is allocated for them)
     device, new = logits_t.device, _empty_strided
     logprob = new((rows,), (1,), dtype=_FP32, device=device) if tokens_t is not None else None
     entropy = new((rows,), (1,), dtype=_FP32, device=device)
-    ids = new((rows, top_k), (top_k, 1), dtype=_INT64, device=device)
-    logprobs = new((rows, top_k), (top_k, 1), dtype=_FP32, device=device)
+    ids = new((rows, room), (room, 1), dtype=_INT64, device=device)
+    logprobs = new((rows, room), (room, 1), dtype=_FP32, device=device)
     _check(lib().uocr_token_logprobs(
         ctx.handle, logits_t.data_ptr(), rows, vocab, between,
         tokens_t.data_ptr() if tokens_t is not None else None, top_k,
