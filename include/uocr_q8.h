@@ -496,7 +496,11 @@ int uocr_kv_export(uocr_ctx *ctx, const uocr_kv *kv, size_t seq, float *keys_out
  * belongs to the device of the context that created it (Invalid with a context
  * of another device) and is used by one stream at a time; all calls but create,
  * free and state are asynchronous on the context's stream, allocate nothing and
- * can be captured in CUDA graphs.
+ * can be captured in CUDA graphs.  The checks of the order of calls and of slots
+ * to read go by the prefills and resets as they are called: a captured one counts
+ * when it is captured, its replays do not (a graph that replays a prefill has the
+ * reset in front of it, and other calls on that sequence expect the tokens of the
+ * prefill that was called last).
  *   uocr_kvq_prefill:  the rows of a prompt into the empty sequence seq;
  *   uocr_kvq_push:     row b of k/v into every sequence b;
  *   uocr_kvq_rope, uocr_kvq_rope_push_qkv: as uocr_kv_rope and
