@@ -213,7 +213,7 @@ void launch_kv_push(float* keys, float* values, int* state, int batch, const KvL
 // copied into sequence b's next slot, then the sequence's counter advances —
 // the same results as uocr_kv_rope followed by uocr_kv_push.
 __global__ void kv_rope_push_kernel(float* keys, float* values, int* state, const KvLayout L,
-                                    int window, const float* __restrict__ qkv, float* q_out,
+                                    int window, const float* qkv, float* q_out,
                                     const float2* __restrict__ table, int max_pos,
                                     unsigned* status) {
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
@@ -233,10 +233,25 @@ __global__ void kv_rope_push_kernel(float* keys, float* values, int* state, cons
   float* qo = q_out + static_cast<long long>(b) * width;
   const bool in_table = pos >= 0 && pos < max_pos;
   if (!in_table && threadIdx.x == 0) flag(status, DEV_POSITION);
-  for (int p = threadIdx.x; p < L.heads * half; p += blockDim.x) {
+  // a thread's next pair of dims is loaded before this one's are stored
+  const int pairs = L.heads * half;
+  float next[6];
+  auto load = [&](int p) {
+    const int d0 = p / half * L.dim + p % half, d1 = d0 + half;
+    next[0] = q[d0];
+    next[1] = q[d1];
+    next[2] = k[d0];
+    next[3] = k[d1];
+    next[4] = v[d0];
+    next[5] = v[d1];
+  };
+  if (threadIdx.x < pairs) load(threadIdx.x);
+  for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
     const int h = p / half, i = p - h * half;
     const int d0 = h * L.dim + i, d1 = d0 + half;
-    float q0 = q[d0], q1 = q[d1], k0 = k[d0], k1 = k[d1];
+    float q0 = next[0], q1 = next[1], k0 = next[2], k1 = next[3];
+    const float v0 = next[4], v1 = next[5];
+    if (p + blockDim.x < pairs) load(p + blockDim.x);
     if (in_table) {
       const float2 cs = table[static_cast<long long>(pos) * half + i];
       const float rq0 = __fsub_rn(__fmul_rn(q0, cs.x), __fmul_rn(q1, cs.y));
@@ -252,8 +267,8 @@ __global__ void kv_rope_push_kernel(float* keys, float* values, int* state, cons
     qo[d1] = q1;
     keys[kv_index(L, b, h, slot, i)] = k0;
     keys[kv_index(L, b, h, slot, i + half)] = k1;
-    values[kv_index(L, b, h, slot, i)] = v[d0];
-    values[kv_index(L, b, h, slot, i + half)] = v[d1];
+    values[kv_index(L, b, h, slot, i)] = v0;
+    values[kv_index(L, b, h, slot, i + half)] = v1;
   }
   __syncthreads();  // every thread has read `gen`
   if (threadIdx.x == 0) state[2 * b + 1] = gen + 1;
@@ -826,7 +841,7 @@ __global__ void __launch_bounds__(kSplitChunk) attn_split_scores_kernel(const At
                                : kh + t * a.row_stride + 32 * j;
         const float4* k4 = reinterpret_cast<const float4*>(row);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) kr[jj * 8 + i] = __ldg(k4 + i);
+        for (int i = 0; i < 8; ++i) kr[jj * 8 + i] = k4[i];
       }
     }
 #pragma unroll

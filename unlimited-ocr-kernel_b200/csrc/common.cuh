@@ -169,8 +169,8 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
 // of 16-float chunk c is stored at index q*C + c (C = n/16 chunks), so when
 // lane l reads part q of chunk l, consecutive lanes read consecutive 16-byte
 // words (no bank conflicts).  n % 16 == 0.
-__device__ __forceinline__ void stage_x_transposed(float* dst, const float* __restrict__ src, int n,
-                                                   int tid, int nthreads) {
+__device__ __forceinline__ void stage_x_transposed(float* dst, const float* src, int n, int tid,
+                                                   int nthreads) {
   const int C = n >> 4;
   const float4* s4 = reinterpret_cast<const float4*>(src);
   float4* d4 = reinterpret_cast<float4*>(dst);
@@ -178,14 +178,14 @@ __device__ __forceinline__ void stage_x_transposed(float* dst, const float* __re
   for (; i + 3 * nthreads < 4 * C; i += 4 * nthreads) {  // 4 loads in flight per thread
     float4 v[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = __ldg(s4 + i + u * nthreads);
+    for (int u = 0; u < 4; ++u) v[u] = s4[i + u * nthreads];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int k = i + u * nthreads;
       d4[(k & 3) * C + (k >> 2)] = v[u];
     }
   }
-  for (; i < 4 * C; i += nthreads) d4[(i & 3) * C + (i >> 2)] = __ldg(s4 + i);
+  for (; i < 4 * C; i += nthreads) d4[(i & 3) * C + (i >> 2)] = s4[i];
 }
 
 // FP32-mode dots of 4 rows of width K (K % 16 == 0) against one x vector
@@ -400,7 +400,10 @@ __device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t by
 // stream (cudaLaunchAttributeProgrammaticStreamSerialization), so that its
 // launch overlaps the previous kernel's end.  The kernel must call
 // pdl_wait_prior_grids() before it reads or writes anything the previous
-// kernel touches (the chain kernels below call it first thing).  Falls back
+// kernel touches (the chain kernels below call it first thing).  What a kernel
+// in front may still write while this one is resident is read by plain loads:
+// the non-coherent path (__ldg, const __restrict__) is for memory that nothing
+// writes during a kernel's whole life, weights and tables.  Falls back
 // to ordinary stream order when the attribute is refused.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,

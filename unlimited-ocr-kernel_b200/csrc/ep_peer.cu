@@ -331,8 +331,8 @@ __global__ void __launch_bounds__(kEpThreads) ep_recv_wait_kernel(const __grid_c
 // token_pos[i] of `rows` (the experts' grouped outputs), or row i when
 // token_pos is null (outputs already in slot order).
 __global__ void __launch_bounds__(kEpThreads) ep_return_kernel(const __grid_constant__ EpDev d,
-                                                               const float* __restrict__ rows,
-                                                               const int* __restrict__ token_pos) {
+                                                               const float* rows,
+                                                               const int* token_pos) {
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -373,29 +373,29 @@ __global__ void __launch_bounds__(kEpThreads) ep_return_kernel(const __grid_cons
 // holds the shared expert's output).  Grid (max(tokens, 1), column blocks of
 // 128 float4); the last CTA advances the step number.
 __global__ void __launch_bounds__(128) ep_combine_kernel(const __grid_constant__ EpDev d,
-                                                         const int32_t* __restrict__ ids,
-                                                         const float* __restrict__ wts, int tokens,
-                                                         float* __restrict__ y) {
+                                                         const int32_t* ids, const float* wts, int tokens,
+                                                         float* y) {
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   const unsigned step = d.ctr[kCtrStep] + 1u;
   const char* own = d.peers[d.rank];
+  const int t = blockIdx.x, k = d.top_k, h4 = d.hidden >> 2;
+  // (this step's own routing: loaded ahead of the wait for the owners)
+  int e[8], p[8];
+  float w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool used = t < tokens && j < k;
+    e[j] = used ? ids[t * k + j] : 0x7fffffff;
+    p[j] = t * k + j;
+    w[j] = used ? wts[t * k + j] : 0.0f;
+    if (used && e[j] < 0) e[j] = 0x7ffffffe;  // an invalid router row (flagged): no pair
+  }
   for (int r = threadIdx.x; r < d.world; r += blockDim.x)
     if (!wait_flag_sys(reinterpret_cast<const unsigned*>(own + d.L.ret_flag) + r, step, d.wait_ns))
       flag(d.status, DEV_TIMEOUT);
   __syncthreads();
-  const int t = blockIdx.x, k = d.top_k, h4 = d.hidden >> 2;
   if (t < tokens) {
-    int e[8], p[8];
-    float w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool used = j < k;
-      e[j] = used ? ids[t * k + j] : 0x7fffffff;
-      p[j] = t * k + j;
-      w[j] = used ? wts[t * k + j] : 0.0f;
-      if (used && e[j] < 0) e[j] = 0x7ffffffe;  // an invalid router row (flagged): no pair
-    }
 #pragma unroll
     for (int i = 1; i < 8; ++i)
 #pragma unroll

@@ -31,7 +31,7 @@ constexpr int kMaxGroupExperts = 256;
 // skip_negative, a negative id marks an unused pair (a padding row of a
 // fixed-capacity dispatch): it joins no group and its token_pos is -1.
 __global__ void __launch_bounds__(kGroupThreads) group_pairs_kernel(
-    const int32_t* __restrict__ ids, const float* __restrict__ wts, int tokens, int top_k,
+    const int32_t* ids, const float* wts, int tokens, int top_k,
     int n_experts, int skip_negative, int* __restrict__ counts, int* __restrict__ offsets,
     int* __restrict__ pair_token, float* __restrict__ pair_weight, int* __restrict__ token_pos,
     int* __restrict__ items, int items_max, unsigned* status) {
@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_pairs_kernel(
   for (int c0 = 0; c0 < npairs; c0 += blockDim.x) {
     const int i = c0 + tid;
     int e = i < npairs ? ids[i] : -1;
+    const float w = i < npairs ? wts[i] : 0.0f;
     if (i < npairs && e < 0 && skip_negative) token_pos[i] = -1;
     const bool valid = i < npairs && !(e < 0 && skip_negative);
     if (valid && (e < 0 || e >= n_experts)) e = 0;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_pairs_kernel(
     if (valid) {
       const int pos = off[e] + cnt[warp][e] + rank;
       pair_token[pos] = i / top_k;
-      pair_weight[pos] = wts[i];
+      pair_weight[pos] = w;
       token_pos[i] = pos;
     }
     __syncthreads();

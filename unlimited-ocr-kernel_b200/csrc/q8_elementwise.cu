@@ -174,7 +174,7 @@ __host__ __device__ inline int bf16_w_stride(int k) { return k + 8; }  // bf16 e
 __host__ __device__ inline int bf16_x_stride(int k) { return k + 4; }  // floats
 
 __global__ void __launch_bounds__(kBf16Threads)
-    linear_bf16_kernel(const uint16_t* __restrict__ w, int n, int k, const float* __restrict__ x,
+    linear_bf16_kernel(const uint16_t* __restrict__ w, int n, int k, const float* x,
                        int batch, float* y, int bulk, unsigned* status) {
   // launched as a programmatic dependent (launch_dependent), nothing touched
   // before the previous kernel completes; no early launch of its own dependents

@@ -324,11 +324,14 @@ __global__ void __launch_bounds__(kSmThreads, 3)
     if (lane == 0) mbar_arrive(&empty[s]);
   }
   // C layout: c0, c1 -> weight row gq, chunk rows 2q, 2q + 1; c2, c3 -> weight row gq + 8
+  float scales[2];  // (both are loaded before the first store)
+#pragma unroll
+  for (int e = 0; e < 2; ++e) scales[e] = INT8 || 2 * q + e >= count ? 1.0f : a.rinv[off + 2 * q + e];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int i = 2 * q + e;
     if (i >= count) continue;
-    const float sc = INT8 ? 1.0f : __ldg(a.rinv + off + i);
+    const float sc = scales[e];
     float* yr = y + (off + i) * a.ldy + n0 + wr0 + gq;
 #pragma unroll
     for (int m = 0; m < 2; ++m)

@@ -909,9 +909,8 @@ constexpr int kSplitMaxV = 8;  // float4 per thread: cols <= 8192
 
 template <bool SWIGLU>
 __global__ void __launch_bounds__(kSplitThreads) split_rows_cta_kernel(
-    const float* __restrict__ x, long long ld_x, const int* __restrict__ src,
-    const float* __restrict__ u, int rows, int cols, uint16_t* __restrict__ pieces,
-    float* __restrict__ rinv, long long piece_elems, const int* __restrict__ live) {
+    const float* x, long long ld_x, const int* src, const float* u, int rows, int cols,
+    uint16_t* __restrict__ pieces, float* __restrict__ rinv, long long piece_elems, const int* live) {
   pdl_launch_dependents();  // launched as a programmatic dependent (launch_dependent):
   pdl_wait_prior_grids();   // nothing is touched before the previous kernel completes
   __shared__ float wmax[kSplitThreads / 32];
