@@ -100,7 +100,7 @@ __device__ __forceinline__ uint32_t kvq_codes4(const float (&x)[4], float m, flo
 }
 
 // The same by the definition, in double (the four divisions in step: a warp that comes
-// here holds up its CTA; one by one they cost 2 us of 78).
+// here holds up its CTA; one by one they cost 2 us more for 32,768 tokens in 8 bits).
 __device__ __noinline__ uint32_t kvq_codes4_exactly(float x0, float x1, float x2, float x3, float m,
                                                     float s, int levels) {
   const float x[4] = {x0, x1, x2, x3};
@@ -155,14 +155,16 @@ void launch_kvq_reset(int* state, int seq, cudaStream_t st) {
 // over eight lanes: halving what a lane keeps at every exchange takes 7 shuffles instead
 // of 24 and leaves the extremes of token u in the lanes u and u + 4 of the eight, which
 // then find its parameters once.
-// Bound by the bytes of the rows and, nearly as much, by issue and the latency of a
-// CTA's load - compute - copy chain: 32,768 tokens of 10 heads of 128 take 70.6 us in 4
-// bits (388 MB: 5.5 TB/s) and 74.3 us in 8 bits (430 MB: 5.8 TB/s), the reset before it
-// counted in.  Persistent CTAs whose rows arrive by asynchronous copies while they work
-// on the last ones were slower (104 against 87 us).
+// Bound by the bytes of the rows and, nearly as much, by issue (70 % of the slots) and
+// the latency of a CTA's load - compute - copy chain: 32,768 tokens of 10 heads of 128
+// take 69.0 us in 4 bits (388 MB: 5.6 TB/s) and 74.3 us in 8 bits (430 MB: 5.8 TB/s),
+// the reset before it counted in.  Six CTAs per SM leave 40 registers and cost 120 to
+// 128 bytes of spills a thread; five CTAs (48 registers, 56 to 104 bytes) take 70.7 and
+// 76.2 us.  An earlier form of 87 us (8 bits) took 104 in
+// persistent CTAs whose rows arrive by asynchronous copies while they work on the last
+// ones.
 // VEC: rows that four floats at a time can be read from, so that a lane's four dims
-// are the row's or not as one.  (Six CTAs per SM, 40 registers; with five 79 us instead
-// of 78, 8 bits, before the last two steps.)
+// are the row's or not as one.
 template <int BITS, bool VEC>
 __global__ void __launch_bounds__(256, 6)
     kvq_prefill_kernel(unsigned char* data, const KvqLayout L, int* state, int seq,
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(256, 6)
           w[i] ^= kvq_flip(BITS);
         }
         // (word i lies 64 i bytes from the first: half of the lanes of a bank take them in
-        // another order, 83 -> 79 us)
+        // another order, 4 us less for 32,768 tokens in 8 bits)
         const bool turn = lane & 8;
         unsigned char* at = codes + kvq_value_byte(half * 16 + j * 4, d0, BITS);
         if (real && (BITS == 8 || !h2)) {
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(256, 6)
       }
     }
   }
-  // the tile leaves as one bulk copy (by vector stores of all threads 87 us, not 79)
+  // the tile leaves as one bulk copy (8 us less than vector stores of all threads)
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
   // (slots past the prompt's end in its last tile get zeros: nothing is in them)
@@ -468,7 +470,8 @@ __device__ __forceinline__ int kvq_tokens(const int* state, int b, int window) {
 // Slots [first, first + count) of one sequence as token-major rows of floats: one CTA
 // per (tile, head), the tile staged in shared memory, lanes as in the prompt's kernel.
 // Bound by the rows written: 32,768 tokens of 10 heads of 128 take 62 us from 4 bits
-// and 69 us from 8 (6.2 and 6.3 TB/s; five CTAs per SM 62 and 71, eight 64 and 73).
+// and 69 us from 8 (6.2 and 6.3 TB/s).  With six CTAs per SM; five took 71 us from 8
+// bits and eight 73.
 template <int BITS, bool VEC>
 __global__ void __launch_bounds__(256, 6)
     kvq_read_kernel(const unsigned char* data, const KvqLayout L, const int* state, int window, int seq,
@@ -576,20 +579,24 @@ void launch_kvq_read(const unsigned char* data, const KvqLayout& L, const int* s
 // of a head (where the heads are few) by the one that ends last.
 //
 // Bound by the cache's bytes where there are many: 64 sequences of 2,176 tokens, 10
-// heads of 128, take 39.3 us in 4 bits (222.8 MB: 5.7 TB/s, 4 us of it the start and
-// the end of a launch) and 62.2 us in 8 bits (401 MB: 6.5 TB/s), 128 sequences of
-// 2,048 tokens 65.7 us in 4 bits (6.4 TB/s); one of 1,645 tokens takes 5.3 us, one of
-// 32,768 tokens 15.4 us (7 us without its bytes).  The same from dequantised values
-// would need some 3 instructions an element, a scheduler's whole rate at this
-// bandwidth; here it is about 1.8 an element (ncu: 54 % of the issue slots).
+// heads of 128, take 39.0 us in 4 bits (222.8 MB: 5.7 TB/s, 4 us of it the start and
+// the end of a launch) and 61.6 us in 8 bits (401 MB: 6.5 TB/s), 128 sequences of
+// 2,048 tokens 65.0 us in 4 bits (6.5 TB/s); one of 1,645 tokens takes 5.5 us, one of
+// 32,768 tokens 15.2 us (7 us without its bytes) and 22.4 us in 8 bits.  The same from
+// dequantised values would need some 3 instructions an element, a scheduler's whole
+// rate at this bandwidth; here it is about 1.7 an element (ncu: 53 % of the issue slots).
+// Not by the tokens of a sequence: the work is split by the cache's capacity and heads,
+// so that one sequence of 32,640 tokens among 63 of 500 takes 170 us in 4 bits (64 of
+// 1,002, as many tokens, 21.5), and 500 tokens 4.4 us in a cache of 2,048 but 8.2 us in
+// one of 32,640.
 // Scores are in powers of two.  They may pass the running maximum by this much.
 constexpr float kKvqSlack = 2.0f;
 // A tile whose scores lie further than this from the maximum that they were summed
 // against is summed again, unless a float at that maximum is too coarse for it.
 constexpr float kKvqFar = 8.0f, kKvqVast = 1048576.0f;
 // Ring slots per warp.  Two tiles in flight for each of 17 warps per SM hide the
-// memory better than more for fewer warps (64 x 2,176 tokens, 4 bits: 2 slots 39.4
-// us, 3 slots 46.2, 4 slots 52.9).
+// memory better than more for fewer warps (64 x 2,176 tokens, 4 bits, as measured when
+// two took 39.4 us: three 46.2, four 52.9).
 constexpr int kKvqSlots = 2;
 constexpr int kKvqCluster = 8;  // most CTAs of a cluster (portable)
 
@@ -602,9 +609,10 @@ __host__ __device__ constexpr int kvq_tile_bytes(int groups, int bits) {
 __host__ __device__ constexpr int kvq_per(int groups, int bits) {
   return kvq_tile_bytes(groups, bits) <= 1280 ? 2 : 1;
 }
-// Warps of a CTA: about 45 KB of shared memory, so that five CTAs share an SM and
-// 740 of them, more than the 640 heads of a batch of 64, run at once (8 bits, 9 KB
-// tiles: two warps 62.4 us, four 71.8).
+// Warps of a CTA, by the bytes of its ring: with 128 dims some 45 KB of shared memory (4
+// bits) and 39 (8), so that five CTAs share an SM and 740 of them, more than the 640
+// heads of a batch of 64, run at once (8 bits, 9 KB tiles: two warps 62.4 us, four
+// 71.8).  Other dims were not swept: 24 to 29 KB at 96 (8 bits) and 160.
 __host__ __device__ constexpr int kvq_warps(int groups, int bits) {
   const int turn = kvq_tile_bytes(groups, bits) * kvq_per(groups, bits);
   return turn <= 5120 ? 4 : turn <= 10240 ? 2 : 1;

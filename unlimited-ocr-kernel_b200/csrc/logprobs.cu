@@ -21,10 +21,12 @@
 // are joined through distributed shared memory.
 //
 // Bound by the logits' bytes where there are many rows: 1517 rows of 129,280 take
-// 119 us without alternatives (6.6 TB/s), 129 us with one, 136 us with twenty.  Few
-// rows are bound by latency, most of it of code that runs once: one row takes 5.4 us
-// without and 9.6 us with twenty alternatives, 64 rows 9.9 us without (their bytes 5
-// us) and 13.9 us with five.
+// 118 us without alternatives (6.6 TB/s), 129 us with one, 137 us with twenty.  Few
+// rows are bound by latency, most of it of code that runs once: one row takes 5.3 us
+// without and 9.7 us with twenty alternatives, 64 rows 9.3 us without (their bytes 5
+// us) and 13.1 us with five.  The second pass is slow: where ten logits of a row are
+// left and the rest are banned, one row takes 33 us with twenty alternatives, 64 rows 75
+// and 1517 rows 988 (with five, which the ten suffice for where a row has one CTA, 136).
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -41,7 +43,7 @@ constexpr int kLpVec = 4;                    // 16-byte vectors per lane and tur
 constexpr int kLpPer = 4 * kLpVec;           // elements per lane and turn
 constexpr int kLpTurn = 32 * kLpVec;         // vectors per warp and turn: one bulk copy
 // Ring slots per warp: two, and four CTAs per SM (1517 rows of 129,280 logits with
-// twenty alternatives, as first built: 152 us; three slots and three CTAs 168, four
+// twenty alternatives, as first built, took 152 us; three slots and three CTAs 168, four
 // and two 176).
 constexpr int kLpStages = 2;
 constexpr int kLpCluster = 8;                // most CTAs per row (portable)

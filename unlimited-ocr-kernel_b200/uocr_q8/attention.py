@@ -216,9 +216,11 @@ def _rows(t, rows, width: int, what: str, device: int):
 
 class QuantizedKvCache:
     """LayerCache for `batch` sequences held in `bits` (4 or 8) bits a dim plus
-    a step and a least value per 32 dims of a head (uocr_kvq): ``KvCache``'s
-    calls, FP32 rows in and out.  Rows of keys and values may lie apart (slices
-    of wider rows)."""
+    a step and a least value per 32 dims of a head (uocr_kvq): the calls of
+    ``KvCache`` with FP32 rows in and out, but for ``attention_prefill`` (a prompt
+    attends to its own rows: ``attention_prefill_device``) and
+    ``set_attention_form``, and ``read`` beside ``export``.  Rows of keys and
+    values may lie apart (slices of wider rows)."""
 
     def __init__(self, ctx: GpuContext, batch: int, heads: int, head_dim: int, window: int,
                  max_prefix: int, bits: int = 4):
