@@ -561,7 +561,8 @@ int uocr_kvq_read(uocr_ctx *ctx, const uocr_kvq *kv, size_t seq, size_t first, s
  * synchronising call; a token id of vocab or above NaN and Shape.  Sums in FP32
  * over at most 512 terms one after the other (in 64 bits above them), the
  * maximum's own term kept apart, so that a nearly certain token's log probability
- * and a nearly zero entropy keep an FP32 relative precision.
+ * and a nearly zero entropy keep a relative precision of 2^-16 (a term e^z, z the
+ * distance from the maximum, is good to 2.25 |z| + 4 steps of 2^-24).
  * Asynchronous on the context's stream; allocates nothing. */
 int uocr_token_logprobs(uocr_ctx *ctx, const float *logits_dev, size_t rows, size_t vocab, size_t ld,
                         const int64_t *tokens_dev, size_t top_k, float *logprob_dev,
